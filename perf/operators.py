@@ -52,12 +52,12 @@ def listed():
         # a large batch of long pairs with an odd length
         {"name": "preference-256x8191", "op": "preference", "pairs": 256, "seq": 8191, "kind": "sigmoid", "smoothing": 0.1,
          "average": False},
-        # the adapters of a 28-layer model, rank 16 (fourteen fp32 tensors per layer)
-        {"name": "clip-392-adapters", "op": "clip", "layers": 28, "hidden": 1536, "inner": 8960, "kv": 256, "rank": 16,
-         "half": False, "norm": "2", "odd": 0},
-        # gradients of wide trainable layers in bf16 beside fp32 ones, odd sizes
-        {"name": "clip-large-mixed", "op": "clip", "layers": 6, "hidden": 4096, "inner": 14336, "kv": 1024, "rank": 512,
-         "half": True, "norm": "2", "odd": 3},
+        # the adapters of a 28-layer model, rank 16 (fourteen fp32 tensors per layer), in one gradient arena
+        {"name": "clip-arena-28-layers", "op": "clip", "layers": 28, "hidden": 1536, "inner": 8960, "kv": 256, "rank": 16,
+         "half": False, "norm": "2", "odd": 0, "arena": True},
+        # a list of 84 gradients of wide trainable layers, bf16 ones beside fp32 ones, odd sizes
+        {"name": "clip-list-84-mixed", "op": "clip", "layers": 6, "hidden": 4096, "inner": 14336, "kv": 1024, "rank": 512,
+         "half": True, "norm": "2", "odd": 3, "arena": False},
     ]
 
 
@@ -85,7 +85,7 @@ def draw(rng):
                 "kind": rng.choice(["sigmoid", "hinge", "ipo"]), "smoothing": rng.choice([0.0, 0.1]), "average": rng.random() < 0.3}
     return {"op": op, "layers": rng.randint(1, 28), "hidden": rng.randint(64, 2048), "inner": rng.randint(64, 8960),
             "kv": rng.randint(16, 512), "rank": _log_uniform(rng, 1, 64), "half": rng.random() < 0.5, "norm": rng.choice(["2", "2", "inf"]),
-            "odd": rng.randint(0, 3)}
+            "odd": rng.randint(0, 3), "arena": rng.random() < 0.3}
 
 
 # ---- inputs --------------------------------------------------------------------------------------------------------
@@ -163,8 +163,8 @@ def prepare(case, seed):
             out, targets = _arena(group, dtype)
             state["flats"].append(flat)
             state["outs"].append(out)
-            state["grads"] += views
-            state["targets"] += targets
+            state["grads"] += [flat] if case["arena"] else views
+            state["targets"] += [out] if case["arena"] else targets
     return state
 
 
