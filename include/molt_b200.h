@@ -314,6 +314,102 @@ int molt_mlp_bwd_t(const molt_lora_proj* gate, const molt_lora_proj* up, const m
                    float* const grads[6], int accumulate, int64_t m, void* workspace, size_t workspace_bytes,
                    uintptr_t stream);
 
+/* ---- preference and policy tuning: token log-probabilities, their losses, gradient clipping ----------------------
+ * The reference trains on next-token cross-entropy alone; these entry points have no counterpart there. */
+
+/* Log-probability of one given token per row of logits [rows, vocab] (dtype MOLT_DTYPE_BF16 or MOLT_DTYPE_F32; row r begins
+ * row_stride * r elements behind the first, row_stride 0 reads one row for all):
+ *   logprob[r] = (x[t] - max) / T - ln(sum_v exp((x[v] - max) / T)),   t = token_ids[r], T = temperature.
+ * A token id outside [0, vocab) (an ignore index such as -100) gives 0 and its row is not read.  Logits of -inf have
+ * probability zero; a row without a finite logit, or with NaN or +inf, gives NaN.  stats (optional): [rows, 2] floats
+ * for molt_token_logprob_bwd (max and log2 of the sum).  fp32 arithmetic. */
+int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, float temperature,
+                           float* logprob, float* stats, int64_t rows, int64_t vocab, uintptr_t stream);
+
+/* grad_logits[r, v] = grad_logprob[r] * (1[v == t] - softmax(x / T)[v]) / T, rounded once; rows whose token id is outside
+ * [0, vocab) get zeros.  grad_logits has the logits' dtype and its own row stride (>= vocab); it may be the logits
+ * themselves (same address and stride) and must not overlap them otherwise. */
+int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, const float* stats,
+                           const float* grad_logprob, float temperature, void* grad_logits, int64_t grad_stride,
+                           int64_t rows, int64_t vocab, uintptr_t stream);
+
+/* Both in one pass over the logits: logprob as molt_token_logprob_fwd, grad_logits as molt_token_logprob_bwd with
+ * grad_logprob[r] = weight[r] (weight NULL: 1).  Meant for a loss whose gradient scales rows: with weight 1 the caller
+ * multiplies by dLoss/dlogprob[r] behind the head's second GEMM, where a row is the hidden width and not the vocabulary. */
+int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, const float* weight,
+                            float temperature, float* logprob, void* grad_logits, int64_t grad_stride, int64_t rows,
+                            int64_t vocab, uintptr_t stream);
+
+#define MOLT_REDUCE_TOKEN 0    /* mean over all kept tokens                                                     */
+#define MOLT_REDUCE_SEQUENCE 1 /* mean over the sequences that keep a token, of the mean over their kept tokens */
+
+/* Clipped policy loss with a KL term over token log-probabilities [batch, seq] (fp32):
+ *   r = exp(logprob - old),  l = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * k,
+ *   k = exp(ref - logprob) - (ref - logprob) - 1,
+ * averaged over the tokens whose mask byte is not zero (mask NULL: all).  Values behind the mask are never used, whatever
+ * they hold.  ref_logprob may be NULL (k = 0).  advantage is [batch, seq] or, with advantage_per_token == 0, [batch].
+ * row_strides: elements between the rows of logprob, old, ref, advantage (between its entries when it is [batch]), mask.
+ * loss[0]; stats[2] = mean k, mean of 1[the clamp cut the gradient].  For the backward (unit_grad NULL: not wanted):
+ * unit_grad [batch, seq] receives d l / d logprob per token, zero behind the mask, and row_weight [batch] the weight of
+ * a kept token of the row.  The clamp's border is decided in 64 bits, sums are kept in 64 bits, in a fixed order. */
+size_t molt_policy_loss_workspace_bytes(int64_t batch, int64_t seq);
+int molt_policy_loss_fwd(const float* logprob, const float* old_logprob, const float* ref_logprob, const float* advantage,
+                         int advantage_per_token, const uint8_t* mask, const int64_t row_strides[5], int64_t batch,
+                         int64_t seq, double clip_low, double clip_high, double kl_coef, int reduction, float* unit_grad,
+                         float* row_weight, float* loss, float* stats, void* workspace, size_t workspace_bytes, uintptr_t stream);
+/* grad_logprob[b, t] = grad_loss[0] * row_weight[b] * unit_grad[b, t] (exactly zero where unit_grad is). */
+int molt_policy_loss_bwd(const float* unit_grad, const float* row_weight, const float* grad_loss, float* grad_logprob,
+                         int64_t batch, int64_t seq, uintptr_t stream);
+
+#define MOLT_PREFERENCE_SIGMOID 0 /* -(1 - smoothing) ln sig(beta h) - smoothing ln sig(-beta h) */
+#define MOLT_PREFERENCE_HINGE 1   /* max(0, 1 - beta h)                                          */
+#define MOLT_PREFERENCE_IPO 2     /* (h - 1 / (2 beta))^2                                        */
+
+/* Loss over `pairs` pairs of sequences: rows 0 .. pairs-1 of logprob [2 * pairs, seq] are the chosen ones, the others the
+ * rejected ones.  s[i] = sum over kept tokens of (logprob - ref) (average != 0: their mean; a row that keeps none: 0),
+ * h[p] = s[p] - s[pairs + p], loss[0] = mean over pairs.  ref_logprob: NULL (0), or with ref_per_token != 0 [2 * pairs, seq],
+ * else [2 * pairs] values subtracted from the rows' sums (their means).  row_strides: of logprob, ref (between entries
+ * when it is [2 * pairs]), mask.  rewards[2 * pairs] = beta * s.  seq_grad[2 * pairs] = d loss / d (a kept token of the row).
+ * Sums are kept in 64 bits, in a fixed order. */
+size_t molt_preference_loss_workspace_bytes(int64_t pairs, int64_t seq);
+int molt_preference_loss_fwd(const float* logprob, const float* ref_logprob, int ref_per_token, const uint8_t* mask,
+                             const int64_t row_strides[3], int64_t pairs, int64_t seq, double beta, double smoothing, int kind,
+                             int average, float* seq_grad, float* rewards, float* loss, void* workspace,
+                             size_t workspace_bytes, uintptr_t stream);
+/* grad_logprob[i, t] = mask[i, t] ? grad_loss[0] * seq_grad[i] : 0, written contiguously. */
+int molt_preference_loss_bwd(const uint8_t* mask, int64_t mask_stride, const float* seq_grad, const float* grad_loss,
+                             float* grad_logprob, int64_t pairs, int64_t seq, uintptr_t stream);
+
+/* One gradient of a list: count elements at grad (device), clipped into out (device; may be grad itself, NULL for the
+ * norm alone).  dtype MOLT_DTYPE_*. */
+typedef struct molt_grad_item {
+  const void* grad;
+  void* out;
+  int64_t count;
+  int64_t dtype;
+} molt_grad_item;
+
+#define MOLT_NORM_L2 0
+#define MOLT_NORM_MAX 1
+
+/* Global norm of a list of gradients (items: array in HOST memory, read before the call returns) and the clipping
+ * coefficient: result[0] = norm of |grad_scale| * g over all elements, result[1] = min(1, max_norm / (result[0] + 1e-6)).
+ * Squares that leave fp32's range are added in 64 bits, so the norm is right for every finite gradient; a NaN or an
+ * infinity reaches result[0].  Same bits for the same list on every call. */
+size_t molt_grad_norm_workspace_bytes(int count);
+int molt_grad_norm(const molt_grad_item* items, int count, int norm_kind, float grad_scale, float max_norm, float* result,
+                   void* workspace, size_t workspace_bytes, uintptr_t stream);
+/* molt_grad_norm with grad_scale 1, and out = grad * result[1] for every item.  Refuses lists whose outputs overlap one
+ * another or another item's gradient. */
+int molt_clip_grads(const molt_grad_item* items, int count, int norm_kind, float max_norm, float* result, void* workspace,
+                    size_t workspace_bytes, uintptr_t stream);
+
+/* molt_adamw_step whose gradients are also multiplied by clip[1], clip being the result of molt_grad_norm with the same
+ * grad_scale (device memory; nothing waits on the host).  A step whose norm clip[0] is not finite changes nothing. */
+int molt_adamw_step_clipped(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count, float lr,
+                            float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
+                            const float* clip, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif

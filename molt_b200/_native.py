@@ -26,6 +26,9 @@ PATH_AUTO, PATH_GENERAL, PATH_TCGEN05, PATH_GEMV, PATH_FEW_TOKENS = 0, 1, 2, 3, 
 PATH_EXACT_DECODE = 0x1000
 PATH_NO_SPLIT, PATH_FORCE_SPLIT, PATH_TALL_TILES, PATH_SHORT_TILES = 0x100, 0x200, 0x400, 0x800   # flags OR-ed onto a path
 OPT_WAIT_LIMIT_US, OPT_WITHHOLD_BLOCKS = 1, 2
+REDUCE_TOKEN, REDUCE_SEQUENCE = 0, 1
+PREFERENCE_SIGMOID, PREFERENCE_HINGE, PREFERENCE_IPO = 0, 1, 2
+NORM_L2, NORM_MAX = 0, 1
 OP_LORA_FWD, OP_LORA_BWD, OP_DX, OP_MLP_FWD, OP_MLP_BWD = 1, 2, 3, 4, 5
 
 EXPORTS = (
@@ -35,7 +38,10 @@ EXPORTS = (
     "molt_add_rmsnorm_bwd", "molt_rope", "molt_adamw_step", "molt_dense_gemm", "molt_nf4_lora_fwd_prepared",
     "molt_nf4_lora_bwd_prepared", "molt_lora_shadow_refresh",
     "molt_dense_gemm_workspace_bytes", "molt_ce_softmax_grad", "molt_mlp_workspace_bytes", "molt_mlp_fwd",
-    "molt_mlp_bwd", "molt_mlp_fwd_t", "molt_mlp_bwd_t",
+    "molt_mlp_bwd", "molt_mlp_fwd_t", "molt_mlp_bwd_t", "molt_token_logprob_fwd", "molt_token_logprob_bwd",
+    "molt_token_logprob_grad", "molt_policy_loss_workspace_bytes", "molt_policy_loss_fwd", "molt_policy_loss_bwd",
+    "molt_preference_loss_workspace_bytes", "molt_preference_loss_fwd", "molt_preference_loss_bwd",
+    "molt_grad_norm_workspace_bytes", "molt_grad_norm", "molt_clip_grads", "molt_adamw_step_clipped",
 )
 
 
@@ -169,6 +175,33 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.molt_mlp_fwd_t.argtypes = [proj, proj, proj, vp, vp, vp, vp, vp, i64, vp, sz, up]
     lib.molt_mlp_bwd_t.restype = i32
     lib.molt_mlp_bwd_t.argtypes = [proj, proj, proj, vp, vp, vp, vp, vp, vp, ctypes.POINTER(vp), i32, i64, vp, sz, up]
+    f64, pi64 = ctypes.c_double, ctypes.POINTER(ctypes.c_int64)
+    lib.molt_token_logprob_fwd.restype = i32
+    lib.molt_token_logprob_fwd.argtypes = [vp, i32, i64, vp, f32, vp, vp, i64, i64, up]
+    lib.molt_token_logprob_bwd.restype = i32
+    lib.molt_token_logprob_bwd.argtypes = [vp, i32, i64, vp, vp, vp, f32, vp, i64, i64, i64, up]
+    lib.molt_token_logprob_grad.restype = i32
+    lib.molt_token_logprob_grad.argtypes = [vp, i32, i64, vp, vp, f32, vp, vp, i64, i64, i64, up]
+    lib.molt_policy_loss_workspace_bytes.restype = sz
+    lib.molt_policy_loss_workspace_bytes.argtypes = [i64, i64]
+    lib.molt_policy_loss_fwd.restype = i32
+    lib.molt_policy_loss_fwd.argtypes = [vp, vp, vp, vp, i32, vp, pi64, i64, i64, f64, f64, f64, i32, vp, vp, vp, vp, vp, sz, up]
+    lib.molt_policy_loss_bwd.restype = i32
+    lib.molt_policy_loss_bwd.argtypes = [vp, vp, vp, vp, i64, i64, up]
+    lib.molt_preference_loss_workspace_bytes.restype = sz
+    lib.molt_preference_loss_workspace_bytes.argtypes = [i64, i64]
+    lib.molt_preference_loss_fwd.restype = i32
+    lib.molt_preference_loss_fwd.argtypes = [vp, vp, i32, vp, pi64, i64, i64, f64, f64, i32, i32, vp, vp, vp, vp, sz, up]
+    lib.molt_preference_loss_bwd.restype = i32
+    lib.molt_preference_loss_bwd.argtypes = [vp, i64, vp, vp, vp, i64, i64, up]
+    lib.molt_grad_norm_workspace_bytes.restype = sz
+    lib.molt_grad_norm_workspace_bytes.argtypes = [i32]
+    lib.molt_grad_norm.restype = i32
+    lib.molt_grad_norm.argtypes = [vp, i32, i32, f32, f32, vp, vp, sz, up]
+    lib.molt_clip_grads.restype = i32
+    lib.molt_clip_grads.argtypes = [vp, i32, i32, f32, vp, vp, sz, up]
+    lib.molt_adamw_step_clipped.restype = i32
+    lib.molt_adamw_step_clipped.argtypes = [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i64, f32, vp, up]
 
 
 def library() -> ctypes.CDLL:

@@ -407,7 +407,12 @@ __global__ void __launch_bounds__(256) rope_kernel(const __nv_bfloat16* q, const
 __global__ void __launch_bounds__(256) adamw_kernel(float4* __restrict__ param, const float4* __restrict__ grad,
                                                     float4* __restrict__ exp_avg, float4* __restrict__ exp_avg_sq,
                                                     long long vectors, float lr, float beta1, float beta2, float eps,
-                                                    float weight_decay, float bias1, float bias2_sqrt, float grad_scale) {
+                                                    float weight_decay, float bias1, float bias2_sqrt, float grad_scale,
+                                                    const float* __restrict__ clip) {
+  if (clip != nullptr) {               // {global norm, clipping coefficient}
+    if (!isfinite(clip[0])) return;    // the step is left out: its gradients would poison both moments
+    grad_scale *= clip[1];
+  }
   for (long long v = blockIdx.x * (long long)blockDim.x + threadIdx.x; v < vectors;
        v += (long long)gridDim.x * blockDim.x) {
     const float4 g4 = __ldcs(grad + v);
@@ -629,14 +634,14 @@ extern "C" int molt_rope(const void* q, const void* k, void* q_out, void* k_out,
   return launch_status("rope_kernel");
 }
 
-extern "C" int molt_adamw_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
-                               float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
-                               float grad_scale, uintptr_t stream) {
-  MOLT_REQUIRE(param && grad && exp_avg && exp_avg_sq, MOLT_E_VALUE, "molt_adamw_step: NULL tensor pointer");
-  MOLT_REQUIRE(count >= 0 && count % 4 == 0, MOLT_E_VALUE, "molt_adamw_step: the element count must be a multiple of 4");
+static int adamw_launch(const char* who, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
+                        float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
+                        const float* clip, uintptr_t stream) {
+  MOLT_REQUIRE(param && grad && exp_avg && exp_avg_sq, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
+  MOLT_REQUIRE(count >= 0 && count % 4 == 0, MOLT_E_VALUE, "%s: the element count must be a multiple of 4", who);
   MOLT_REQUIRE(aligned16(param) && aligned16(grad) && aligned16(exp_avg) && aligned16(exp_avg_sq), MOLT_E_VALUE,
-               "molt_adamw_step: arrays must be 16-byte aligned");
-  MOLT_REQUIRE(step >= 1, MOLT_E_VALUE, "molt_adamw_step: step counts from 1");
+               "%s: arrays must be 16-byte aligned", who);
+  MOLT_REQUIRE(step >= 1, MOLT_E_VALUE, "%s: step counts from 1", who);
   if (count == 0) return MOLT_OK;
   const double bias1 = 1.0 - pow((double)beta1, (double)step);
   const double bias2 = 1.0 - pow((double)beta2, (double)step);
@@ -644,8 +649,23 @@ extern "C" int molt_adamw_step(float* param, const float* grad, float* exp_avg, 
   adamw_kernel<<<grid_for(vectors, 256, 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       reinterpret_cast<float4*>(param), reinterpret_cast<const float4*>(grad), reinterpret_cast<float4*>(exp_avg),
       reinterpret_cast<float4*>(exp_avg_sq), vectors, lr, beta1, beta2, eps, weight_decay, (float)bias1,
-      (float)sqrt(bias2), grad_scale);
+      (float)sqrt(bias2), grad_scale, clip);
   return launch_status("adamw_kernel");
+}
+
+extern "C" int molt_adamw_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
+                               float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
+                               float grad_scale, uintptr_t stream) {
+  return adamw_launch("molt_adamw_step", param, grad, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, weight_decay, step,
+                      grad_scale, nullptr, stream);
+}
+
+extern "C" int molt_adamw_step_clipped(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
+                                       float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
+                                       float grad_scale, const float* clip, uintptr_t stream) {
+  MOLT_REQUIRE(clip != nullptr, MOLT_E_VALUE, "molt_adamw_step_clipped: clip is NULL");
+  return adamw_launch("molt_adamw_step_clipped", param, grad, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, weight_decay,
+                      step, grad_scale, clip, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -1,0 +1,110 @@
+"""Global gradient norm over many tensors, and clipping (``molt_grad_norm``, ``molt_clip_grads``): what stands between a
+backward pass and the optimizer step.  Nothing is read back to the host."""
+from __future__ import annotations
+
+from array import array
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from molt_b200 import _native
+from molt_b200.core.errors import CapabilityError
+
+_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
+_NORMS = {2.0: _native.NORM_L2, float("inf"): _native.NORM_MAX}
+
+Grads = Union[torch.Tensor, Sequence[torch.Tensor]]
+
+
+def _dense(tensor: torch.Tensor) -> bool:
+    """Whether the elements fill one stretch of memory, in whatever order."""
+    expect = 1
+    for extent, stride in sorted(zip(tensor.shape, tensor.stride()), key=lambda p: (p[1], p[0])):
+        if extent != 1:
+            if stride != expect:
+                return False
+            expect *= extent
+    return True
+
+
+def _checked(name: str, tensors: Grads) -> Tuple[torch.Tensor, ...]:
+    tensors = (tensors,) if isinstance(tensors, torch.Tensor) else tuple(tensors)
+    if not tensors:
+        raise ValueError(f"{name}: at least one tensor is needed")
+    if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.numel() == 0 or _dense(t) for t in tensors):
+        raise ValueError(f"{name}: every tensor must fill its memory (no gaps, no repeated elements)")
+    return tensors
+
+
+def _norm_kind(norm_type: float) -> int:
+    kind = _NORMS.get(float(norm_type))
+    if kind is None:
+        raise CapabilityError("the gradient norm is 2 or inf")
+    return kind
+
+
+def _items(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]]) -> array:
+    """The list as ``molt_grad_item`` records."""
+    if len(set(map(torch.Tensor.get_device, grads))) != 1 or grads[0].device.type != "cuda":
+        if any(t.device.type != "cuda" for t in grads):
+            raise CapabilityError("gradient norms require CUDA tensors")
+        raise ValueError("all gradients must be on one device")
+    try:
+        dtypes = [_DTYPES[t.dtype] for t in grads]
+    except KeyError:
+        raise CapabilityError("gradient norms support bfloat16 and float32 tensors") from None
+    count = len(grads)
+    flat = [0] * (4 * count)
+    flat[0::4] = map(torch.Tensor.data_ptr, grads)
+    if outs is not None:
+        flat[1::4] = flat[0::4] if outs is grads else map(torch.Tensor.data_ptr, outs)
+    flat[2::4] = map(torch.Tensor.numel, grads)
+    flat[3::4] = dtypes
+    return array("q", flat)
+
+
+@torch.no_grad()
+def global_grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
+    """Norm of all elements of ``grads`` (one tensor or a sequence; bf16 and fp32 may be mixed) as an fp32 scalar on the
+    device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  It is right for every
+    finite gradient, however large or small; a NaN gives NaN, and an infinity infinity.  Equal lists give equal bits."""
+    grads = _checked("grads", grads)
+    kind = _norm_kind(norm_type)
+    items = _items(grads, None)
+    device = grads[0].device
+    lib = _native.library()
+    scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(len(grads)), device)
+    result = torch.empty(2, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        _native.check(lib.molt_grad_norm(items.buffer_info()[0], len(grads), kind, 1.0, float("inf"), result.data_ptr(),
+                                         scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
+    return result[0]
+
+
+@torch.no_grad()
+def clip_grad_norm(grads: Grads, max_norm: float, norm_type: float = 2.0, out: Optional[Grads] = None) -> torch.Tensor:
+    """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return their :func:`global_grad_norm` before that.
+
+    In place, or into ``out`` (tensors like ``grads``; an output may be its own gradient but must not overlap another
+    tensor of the call).  One tensor must not stand in the list twice."""
+    grads = _checked("grads", grads)
+    kind = _norm_kind(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must not be negative")
+    outs = grads if out is None else _checked("out", out)
+    if outs is not grads:
+        if len(outs) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device
+                                          for o, g in zip(outs, grads)):
+            raise ValueError("out must match grads in number, shape, dtype and device")
+        if any(o.stride() != g.stride() for o, g in zip(outs, grads) if not (o.is_contiguous() and g.is_contiguous())):
+            raise ValueError("out must lie in memory as grads do")
+    items = _items(grads, outs)
+    device = grads[0].device
+    lib = _native.library()
+    scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(len(grads)), device)
+    result = torch.empty(2, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        _native.check(lib.molt_clip_grads(items.buffer_info()[0], len(grads), kind, float(max_norm), result.data_ptr(),
+                                          scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
+    torch.autograd.graph.increment_version(outs)
+    return result[0]

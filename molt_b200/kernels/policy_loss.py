@@ -1,0 +1,205 @@
+"""Losses over token log-probabilities for preference and policy tuning: the clipped policy loss with a KL term
+(``molt_policy_loss_*``) and the loss over pairs of sequences (``molt_preference_loss_*``).  Forward and backward are
+CUDA kernels; the reference, which trains on cross-entropy alone, has no counterpart."""
+from __future__ import annotations
+
+import ctypes
+from typing import Any, NamedTuple, Optional
+
+import torch
+
+from molt_b200 import _native
+from molt_b200.core.errors import CapabilityError
+
+_REDUCTIONS = {"token": _native.REDUCE_TOKEN, "sequence": _native.REDUCE_SEQUENCE}
+_KINDS = {"sigmoid": _native.PREFERENCE_SIGMOID, "hinge": _native.PREFERENCE_HINGE, "ipo": _native.PREFERENCE_IPO}
+
+
+class PolicyLoss(NamedTuple):
+    """Scalars on the device; only ``loss`` carries a gradient."""
+
+    loss: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+class PreferenceLoss(NamedTuple):
+    """``loss`` is a scalar that carries the gradient, the rewards are ``[pairs]``."""
+
+    loss: torch.Tensor
+    chosen_rewards: torch.Tensor
+    rejected_rewards: torch.Tensor
+
+
+def _check_logprobs(who: str, logprobs: torch.Tensor) -> None:
+    if logprobs.device.type != "cuda":
+        raise CapabilityError(f"{who} requires CUDA tensors")
+    if logprobs.dtype != torch.float32:
+        raise CapabilityError(f"{who} requires float32 log-probabilities")
+    if logprobs.dim() != 2:
+        raise ValueError("logprobs must be [sequences, tokens]")
+
+
+def _check_like(name: str, tensor: torch.Tensor, logprobs: torch.Tensor, shape) -> None:
+    if tensor.shape != shape or tensor.dtype != torch.float32 or tensor.device != logprobs.device:
+        raise ValueError(f"{name} must be float32 of shape {tuple(shape)} on the device of logprobs")
+
+
+def _check_mask(mask: Optional[torch.Tensor], logprobs: torch.Tensor) -> None:
+    if mask is not None and (mask.shape != logprobs.shape or mask.dtype not in (torch.bool, torch.uint8)
+                             or mask.device != logprobs.device):
+        raise ValueError("mask must be bool or uint8 of the shape and on the device of logprobs")
+
+
+def _rows(tensor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The tensor, or a copy where its rows overlap or its tokens are not neighbours (rows may be one and the same)."""
+    if tensor is None or tensor.dim() == 1:
+        return tensor
+    rows, width = tensor.shape
+    neighbours = width <= 1 or tensor.stride(1) == 1
+    apart = rows <= 1 or tensor.stride(0) == 0 or tensor.stride(0) >= width
+    return tensor if neighbours and apart else tensor.contiguous()
+
+
+def _row_stride(tensor: Optional[torch.Tensor]) -> int:
+    if tensor is None or tensor.shape[0] <= 1:
+        return 0
+    return tensor.stride(0)
+
+
+class _PolicyLossFunction(torch.autograd.Function):
+    """Keeps one fp32 value per token and one per sequence for the backward pass."""
+
+    @staticmethod
+    def forward(ctx: Any, logprobs, old, ref, advantages, mask, clip_low, clip_high, kl_coef, reduction):
+        batch, seq = logprobs.shape
+        lp, old, ref, mask = _rows(logprobs), _rows(old), _rows(ref), _rows(mask)
+        advantages = _rows(advantages)
+        device = lp.device
+        trained = ctx.needs_input_grad[0]
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        stats = torch.empty(2, dtype=torch.float32, device=device)
+        unit = torch.empty((batch, seq), dtype=torch.float32, device=device) if trained else None
+        weight = torch.empty(batch, dtype=torch.float32, device=device) if trained else None
+        lib = _native.library()
+        scratch = _native.workspace(lib.molt_policy_loss_workspace_bytes(batch, seq), device)
+        strides = (ctypes.c_int64 * 5)(*map(_row_stride, (lp, old, ref, advantages, mask)))
+        with torch.cuda.device(device):
+            _native.check(lib.molt_policy_loss_fwd(
+                lp.data_ptr(), old.data_ptr(), _native.ptr(ref), advantages.data_ptr(), int(advantages.dim() == 2),
+                _native.ptr(mask), strides, batch, seq, clip_low, clip_high, kl_coef, reduction, _native.ptr(unit),
+                _native.ptr(weight), loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), scratch.numel(),
+                _native.stream_handle(device)))
+        if trained:
+            ctx.save_for_backward(unit, weight)
+        kl, cut = stats[0], stats[1]
+        ctx.mark_non_differentiable(kl, cut)
+        ctx.set_materialize_grads(False)
+        return loss, kl, cut
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, grad_loss, grad_kl, grad_cut):
+        unit, weight = ctx.saved_tensors
+        grad = torch.empty_like(unit)
+        grad_loss = grad_loss.float().contiguous()
+        with torch.cuda.device(unit.device):
+            _native.check(_native.library().molt_policy_loss_bwd(
+                unit.data_ptr(), weight.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(), unit.shape[0], unit.shape[1],
+                _native.stream_handle(unit.device)))
+        return grad, None, None, None, None, None, None, None, None
+
+
+def clipped_policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                        mask: Optional[torch.Tensor] = None, ref_logprobs: Optional[torch.Tensor] = None,
+                        clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
+                        reduction: str = "token") -> PolicyLoss:
+    """Mean over tokens of ``-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k`` with
+    ``r = exp(logprobs - old_logprobs)`` and ``k = exp(ref - logprobs) - (ref - logprobs) - 1``.
+
+    ``logprobs``, ``old_logprobs`` and ``ref_logprobs`` are fp32 ``[sequences, tokens]``, ``advantages`` the same or
+    ``[sequences]``.  Only tokens with a true ``mask`` count; what stands behind the mask is never used, NaN included.
+    ``reduction="token"`` averages over all kept tokens, ``"sequence"`` over the sequences that keep one, of the mean over
+    their kept tokens.  Without a kept token the loss and its gradient are zero.  Returns the loss, the mean ``k`` and the
+    mean share of tokens whose gradient the clamp cut.  Only ``logprobs`` gets a gradient; a log-ratio on the clamp's
+    border keeps its own."""
+    _check_logprobs("clipped_policy_loss", logprobs)
+    _check_like("old_logprobs", old_logprobs, logprobs, logprobs.shape)
+    if ref_logprobs is not None:
+        _check_like("ref_logprobs", ref_logprobs, logprobs, logprobs.shape)
+    _check_like("advantages", advantages, logprobs, logprobs.shape if advantages.dim() == 2 else logprobs.shape[:1])
+    _check_mask(mask, logprobs)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    return PolicyLoss(*_PolicyLossFunction.apply(logprobs, old_logprobs.detach(),
+                                                 None if ref_logprobs is None else ref_logprobs.detach(), advantages.detach(),
+                                                 mask, float(clip_low), float(clip_high), float(kl_coef),
+                                                 _REDUCTIONS[reduction]))
+
+
+class _PreferenceLossFunction(torch.autograd.Function):
+    """Keeps the mask and one fp32 value per sequence for the backward pass."""
+
+    @staticmethod
+    def forward(ctx: Any, logprobs, ref, mask, beta, smoothing, kind, average):
+        sequences, seq = logprobs.shape
+        pairs = sequences // 2
+        lp, mask = _rows(logprobs), _rows(mask)
+        ref = _rows(ref)
+        device = lp.device
+        trained = ctx.needs_input_grad[0]
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        rewards = torch.empty((2, pairs), dtype=torch.float32, device=device)
+        seq_grad = torch.empty(sequences, dtype=torch.float32, device=device) if trained else None
+        lib = _native.library()
+        scratch = _native.workspace(lib.molt_preference_loss_workspace_bytes(pairs, seq), device)
+        strides = (ctypes.c_int64 * 3)(*map(_row_stride, (lp, ref, mask)))
+        with torch.cuda.device(device):
+            _native.check(lib.molt_preference_loss_fwd(
+                lp.data_ptr(), _native.ptr(ref), int(ref is not None and ref.dim() == 2), _native.ptr(mask), strides, pairs, seq,
+                beta, smoothing, kind, average, _native.ptr(seq_grad), rewards.data_ptr(), loss.data_ptr(), scratch.data_ptr(),
+                scratch.numel(), _native.stream_handle(device)))
+        if trained:
+            ctx.save_for_backward(mask, seq_grad)
+            ctx.seq = seq
+        chosen, rejected = rewards[0], rewards[1]
+        ctx.mark_non_differentiable(chosen, rejected)
+        ctx.set_materialize_grads(False)
+        return loss, chosen, rejected
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, grad_loss, grad_chosen, grad_rejected):
+        mask, seq_grad = ctx.saved_tensors
+        grad = torch.empty((seq_grad.shape[0], ctx.seq), dtype=torch.float32, device=seq_grad.device)
+        grad_loss = grad_loss.float().contiguous()
+        with torch.cuda.device(grad.device):
+            _native.check(_native.library().molt_preference_loss_bwd(
+                _native.ptr(mask), _row_stride(mask), seq_grad.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(),
+                grad.shape[0] // 2, ctx.seq, _native.stream_handle(grad.device)))
+        return grad, None, None, None, None, None, None
+
+
+def preference_loss(logprobs: torch.Tensor, ref_logprobs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                    beta: float = 0.1, label_smoothing: float = 0.0, kind: str = "sigmoid",
+                    average: bool = False) -> PreferenceLoss:
+    """Loss over pairs of sequences from their token log-probabilities (fp32 ``[2 * pairs, tokens]``: the chosen sequences,
+    then the rejected ones in the same order).
+
+    With ``s`` the sum over a sequence's kept tokens of ``logprobs - ref_logprobs`` (``average``: their mean) and
+    ``h = s_chosen - s_rejected``, the mean over pairs of ``-(1 - e) ln sig(beta h) - e ln sig(-beta h)`` for ``"sigmoid"``
+    (``e`` the label smoothing), ``max(0, 1 - beta h)`` for ``"hinge"``, ``(h - 1 / (2 beta))^2`` for ``"ipo"``.
+    ``ref_logprobs`` is ``[2 * pairs, tokens]``, or ``[2 * pairs]`` sums (means with ``average``) kept from an earlier pass, or
+    None (zero).  What stands behind the mask is never used; a sequence that keeps no token has ``s = 0``.  The rewards
+    are ``beta s``.  Only ``logprobs`` gets a gradient."""
+    _check_logprobs("preference_loss", logprobs)
+    if logprobs.shape[0] == 0 or logprobs.shape[0] % 2:
+        raise ValueError("logprobs must hold the chosen sequences and then as many rejected ones")
+    if ref_logprobs is not None:
+        _check_like("ref_logprobs", ref_logprobs, logprobs,
+                    logprobs.shape if ref_logprobs.dim() == 2 else logprobs.shape[:1])
+    _check_mask(mask, logprobs)
+    if kind not in _KINDS:
+        raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+    return PreferenceLoss(*_PreferenceLossFunction.apply(logprobs, None if ref_logprobs is None else ref_logprobs.detach(), mask,
+                                                         float(beta), float(label_smoothing), _KINDS[kind], int(bool(average))))
