@@ -15,88 +15,353 @@ __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-// The running pair (maximum m, sum s of exp2((x - m) c)) of two parts joined.  A part without a finite logit has m = -inf
-// and s = 0; NaN logits leave NaN in s.
-__device__ __forceinline__ void join(float& m, float& s, float om, float os, float c) {
-  const float nm = fmaxf(m, om);
-  const float a = m == nm ? s : s * exp2f((m - nm) * c);
-  const float b = om == nm ? os : os * exp2f((om - nm) * c);
-  m = nm;
-  s = a + b;
+__device__ __forceinline__ float exp2_fast(float v) {   // 2^-22 relative
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-constexpr int kThreads = 512;
+// Pairs of fp32 in one 64-bit register: one instruction for two additions, products or fused products.
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair(float a, float b) {
+  pair_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(pair_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+  pair_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ pair_t exp2_2(pair_t v) {
+  const float2 h = halves(v);
+  return pair(exp2_fast(h.x), exp2_fast(h.y));
+}
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kThreads) row_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids,
-                                                       const float* __restrict__ weight, float inv_t, float* __restrict__ logprob,
-                                                       float2* __restrict__ stats, T* grad, long long grad_stride, int vocab) {
-  __shared__ float part_m[kThreads / 32], part_s[kThreads / 32];
-  const long long row = blockIdx.x, t = ids[row];
-  const T* x = logits + row * row_stride;
-  T* g = GRAD ? grad + row * grad_stride : nullptr;
-  if (t < 0 || t >= vocab) {
-    if (threadIdx.x == 0) {
-      logprob[row] = 0.f;
-      if (stats != nullptr) stats[row] = make_float2(0.f, 0.f);
-    }
-    if (GRAD)
-      for (int v = threadIdx.x; v < vocab; v += kThreads) store1(g + v, 0.f);
-    return;
+// What the kernels need of 16 bytes of logits.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kElements = 4;
+  static __device__ __forceinline__ float largest(const uint4& q, float m) {
+    return fmaxf(fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w))), m);
   }
-  const float c = inv_t * kLog2e;
-  float m = -INFINITY, s = 0.f;
-  for (int v = threadIdx.x; v < vocab; v += kThreads) {
-    const float xv = load1(x + v);
-    if (xv == -INFINITY) continue;   // probability zero
-    join(m, s, xv, 1.f, c);
-    if (isnan(xv)) s = xv;
+  template <typename F>
+  static __device__ __forceinline__ void each(const uint4& q, F f) {
+    f(0, pair(__uint_as_float(q.x), __uint_as_float(q.y)));
+    f(1, pair(__uint_as_float(q.z), __uint_as_float(q.w)));
   }
-  const float xt = load1(x + t);
+  template <typename F>
+  static __device__ __forceinline__ uint4 map(const uint4& q, F f) {
+    const float2 a = halves(f(pair(__uint_as_float(q.x), __uint_as_float(q.y))));
+    const float2 b = halves(f(pair(__uint_as_float(q.z), __uint_as_float(q.w))));
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int kElements = 8;
+  static __device__ __forceinline__ unsigned max2(unsigned a, unsigned b) {   // drops a NaN, which the sum then carries
+    unsigned r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float largest(const uint4& q, float m) {
+    const unsigned v = max2(max2(q.x, q.y), max2(q.z, q.w));
+    return fmaxf(m, fmaxf(bf16_lo(v), bf16_hi(v)));
+  }
+  template <typename F>
+  static __device__ __forceinline__ void each(const uint4& q, F f) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
-  if ((threadIdx.x & 31) == 0) {
-    part_m[threadIdx.x >> 5] = m;
-    part_s[threadIdx.x >> 5] = s;
+    for (int i = 0; i < 4; ++i) f(i, pair(bf16_lo(w[i]), bf16_hi(w[i])));
   }
+  template <typename F>
+  static __device__ __forceinline__ uint4 map(const uint4& q, F f) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+    unsigned o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 h = halves(f(pair(bf16_lo(w[i]), bf16_hi(w[i]))));
+      o[i] = pack_bf16x2(h.x, h.y);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
+};
+
+// ---- the running pair (maximum m, sum s of exp2((x - m) c)) -----------------------------------------------------------
+// A part without a finite logit has m = -inf and s = 0; a NaN logit leaves NaN in s; m = +inf makes inf - inf in s.
+struct Running {
+  float m = -INFINITY;
+  pair_t s = 0;   // two partial sums
+  float c;
+
+  // What the exponents are taken from: -inf - -inf must not arise while only -inf has been seen.
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+  __device__ __forceinline__ void raise(float to) {
+    const float before = m;
+    m = to;
+    const float k = exp2_fast((before - base()) * c);
+    s = mul2(s, pair(k, k));
+  }
+  template <typename T, int N>
+  __device__ __forceinline__ void take(const uint4 (&q)[N]) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = Vec<T>::largest(q[j], top);
+    raise(top);
+    const float from = -base();
+    const pair_t minus = pair(from, from), cc = pair(c, c);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      Vec<T>::each(q[j], [&](int, pair_t x) { s = add2(s, exp2_2(mul2(add2(x, minus), cc))); });
+  }
+  __device__ __forceinline__ void take_one(float x) {
+    raise(fmaxf(m, x));
+    s = add2(s, pair(exp2_fast((x - base()) * c), 0.f));
+  }
+};
+
+__device__ __forceinline__ void warp_join(float& m, float& s, float c) {
+  float top = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  s = m == top ? s : s * exp2_fast((m - top) * c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  m = top;
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_in_cta(float2* slot, unsigned cta, float2 v) {
+  const unsigned local = (unsigned)__cvta_generic_to_shared(slot);
+  unsigned remote;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(cta));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
+}
+
+// Joins the pairs of all threads that share a row; every thread gets the result.  The caller's cluster has arrived at the
+// cluster barrier once (so that every block's shared memory exists before another block writes to it).
+template <int THREADS>
+__device__ __forceinline__ void row_join(float& m, float& s, float c, unsigned rank, unsigned size) {
+  __shared__ float2 of_warp[32], of_cta[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  warp_join(m, s, c);
+  if (lane == 0) of_warp[warp] = make_float2(m, s);
   __syncthreads();
-  m = part_m[0];
-  s = part_s[0];
-  for (int w = 1; w < kThreads / 32; ++w) join(m, s, part_m[w], part_s[w], c);
-  if (m == INFINITY) s = NAN;
-  const float log2_s = log2f(s);
-  const float l = (xt - m) * inv_t - log2_s * kLn2;
-  if (threadIdx.x == 0) {
-    logprob[row] = l;
-    if (stats != nullptr) stats[row] = make_float2(m, log2_s);
+  float2 q = lane < THREADS / 32 ? of_warp[lane] : make_float2(-INFINITY, 0.f);
+  m = q.x;
+  s = q.y;
+  warp_join(m, s, c);
+  if (size > 1) {
+    cluster_wait();
+    if (warp == 0 && lane < size) store_in_cta(of_cta + rank, lane, make_float2(m, s));
+    cluster_arrive();
+    cluster_wait();
+    q = lane < size ? of_cta[lane] : make_float2(-INFINITY, 0.f);
+    m = q.x;
+    s = q.y;
+    warp_join(m, s, c);
   }
-  if (GRAD) {
-    const float w = (weight != nullptr ? weight[row] : 1.f) * inv_t;
-    __syncthreads();   // the target's logit has been read by all before it may be overwritten
-    for (int v = threadIdx.x; v < vocab; v += kThreads)
-      store1(g + v, v == t ? -expm1f(l) * w : -exp2f((load1(x + v) - m) * c - log2_s) * w);
+}
+
+// Where a row's 16-byte vectors begin and how many there are; `head` elements stand in front of them, `tail` behind.
+template <typename T>
+struct Cut {
+  int head, vectors, tail;
+  __device__ __forceinline__ Cut(const T* x, int vocab) {
+    constexpr int E = Vec<T>::kElements;
+    head = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
+    if (head > vocab) head = vocab;
+    vectors = (vocab - head) / E;
+    tail = vocab - head - vectors * E;
+  }
+  // Element outside the vectors that thread `i` looks after (the first 8 threads in front, the next 8 behind), or -1.
+  __device__ __forceinline__ int loose(int i, int vocab) const {
+    return i < 8 ? (i < head ? i : -1) : (i < 16 && i - 8 < tail ? vocab - tail + i - 8 : -1);
+  }
+};
+
+// Zeros for elements [begin, end), by `count` threads of which this is thread `i`.
+template <typename T>
+__device__ __forceinline__ void clear(T* g, int begin, int end, int i, int count) {
+  const Cut<T> cut(g + begin, end - begin);
+  const int own = i < 16 ? cut.loose(i, end - begin) : -1;
+  if (own >= 0) store1(g + begin + own, 0.f);
+  uint4* p = reinterpret_cast<uint4*>(g + begin + cut.head);
+  for (int v = i; v < cut.vectors; v += count) __stcs(p + v, make_uint4(0, 0, 0, 0));
+}
+
+// A vector of gradients to elements that begin at `g`: one store where the gradient is cut like the logits.
+template <typename T>
+__device__ __forceinline__ void put(T* g, const uint4& q, bool same_cut) {
+  if (same_cut) {
+    __stcs(reinterpret_cast<uint4*>(g), q);
+  } else {
+    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::kElements; ++i) g[i] = e[i];
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const T* logits, long long row_stride,
-                                                            const long long* __restrict__ ids,
-                                                            const float2* __restrict__ stats,
-                                                            const float* __restrict__ grad_logprob, float inv_t, T* grad,
-                                                            long long grad_stride, int vocab) {
-  const long long row = blockIdx.x, t = ids[row];
+__device__ __forceinline__ bool cut_alike(const T* a, const T* b) {
+  return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+
+// One row per cluster of blocks (of one block, when there are enough rows).  First pass: the running pair over the
+// block's vectors, NB of them at a time.  GRAD: second pass, from the last vector to the first, over the same vectors, which
+// the L2 still holds.
+template <typename T, bool GRAD, int THREADS, int NB, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
+    row_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids, const float* __restrict__ weight,
+               float inv_t, float* __restrict__ logprob, float2* __restrict__ stats, T* grad, long long grad_stride, int vocab) {
+  constexpr int E = Vec<T>::kElements;
+  const unsigned size = cluster_size(), rank = cluster_rank();
+  const long long row = blockIdx.x / size, t = ids[row];
   const T* x = logits + row * row_stride;
-  T* g = grad + row * grad_stride;
+  T* g = GRAD ? grad + row * grad_stride : nullptr;
+  const int first = rank * THREADS + threadIdx.x, step = size * THREADS;
   if (t < 0 || t >= vocab) {
-    for (int v = threadIdx.x; v < vocab; v += kThreads) store1(g + v, 0.f);
+    if (first == 0) {
+      logprob[row] = 0.f;
+      if (!GRAD && stats != nullptr) stats[row] = make_float2(0.f, 0.f);
+    }
+    if (GRAD) clear(g, 0, vocab, first, step);
     return;
   }
-  const float c = inv_t * kLog2e, m = stats[row].x, log2_s = stats[row].y;
-  const float w = grad_logprob[row] * inv_t;
-  for (int v = threadIdx.x; v < vocab; v += kThreads) {
-    const float d = load1(x + v) - m;
-    store1(g + v, v == t ? -expm1f(d * inv_t - log2_s * kLn2) * w : -exp2f(d * c - log2_s) * w);
+  if (size > 1) cluster_arrive();
+  const Cut<T> cut(x, vocab);
+  const uint4* p = reinterpret_cast<const uint4*>(x + cut.head);
+  const int loose = first < 16 ? cut.loose(first, vocab) : -1;
+  const float xt = load1(x + t);
+  Running run;
+  run.c = inv_t * kLog2e;
+  int v = first;
+  for (; v + (NB - 1) * step < cut.vectors; v += NB * step) {
+    uint4 q[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) q[j] = GRAD ? p[v + j * step] : __ldcs(p + v + j * step);
+    run.template take<T, NB>(q);
+  }
+  const int whole = v;
+  for (; v < cut.vectors; v += step) {
+    const uint4 q[1] = {GRAD ? p[v] : __ldcs(p + v)};
+    run.template take<T, 1>(q);
+  }
+  float loose_x = 0.f;
+  if (loose >= 0) {
+    loose_x = load1(x + loose);
+    run.take_one(loose_x);
+  }
+  const float2 sums = halves(run.s);
+  float m = run.m, s = sums.x + sums.y;
+  row_join<THREADS>(m, s, run.c, rank, size);
+  const float log2_s = log2f(s);
+  const float l = (xt - m) * inv_t - log2_s * kLn2;
+  if (first == 0) {
+    logprob[row] = l;
+    if (!GRAD && stats != nullptr) stats[row] = make_float2(m, log2_s);
+  }
+  if (GRAD) {
+    const float w = (weight != nullptr ? weight[row] : 1.f) * inv_t;
+    const pair_t minus = pair(-m, -m), cc = pair(run.c, run.c), less = pair(-log2_s, -log2_s), scale = pair(-w, -w);
+    const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
+    const bool alike = cut_alike(x, g);
+    T* to = g + cut.head;
+    for (v -= step; v >= whole; v -= step) put(to + (long long)v * E, Vec<T>::map(__ldcs(p + v), f), alike);
+    for (v = whole - NB * step; v >= 0; v -= NB * step) {
+      uint4 q[NB];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) q[j] = __ldcs(p + v + j * step);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) put(to + (long long)(v + j * step) * E, Vec<T>::map(q[j], f), alike);
+    }
+    if (loose >= 0) store1(g + loose, exp2_fast((loose_x - m) * run.c - log2_s) * -w);
+    // the target's own column, by the thread that has just written it: 1 - p without the cancellation
+    const int at = (int)t - cut.head, holder = at / E;
+    const bool own = at >= 0 && holder < cut.vectors ? holder % step == first : loose == (int)t;
+    if (own) store1(g + t, -expm1f(l) * w);
+  }
+}
+
+// A block takes 4 vectors per thread of one row: no loop, many blocks, reads and writes spread evenly.
+constexpr int kBackThreads = 256, kBackVectors = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits, long long row_stride,
+                                                                const long long* __restrict__ ids,
+                                                                const float2* __restrict__ stats,
+                                                                const float* __restrict__ grad_logprob, float inv_t, T* grad,
+                                                                long long grad_stride, int vocab, int parts) {
+  constexpr int E = Vec<T>::kElements, kPart = kBackThreads * kBackVectors;
+  const long long row = blockIdx.x / parts, t = ids[row];
+  const int part = blockIdx.x - row * parts;
+  const T* x = logits + row * row_stride;
+  T* g = grad + row * grad_stride;
+  const Cut<T> cut(x, vocab);
+  const bool last = part == parts - 1;
+  if (t < 0 || t >= vocab) {
+    clear(g, part == 0 ? 0 : min(vocab, cut.head + part * kPart * E), last ? vocab : min(vocab, cut.head + (part + 1) * kPart * E),
+          threadIdx.x, kBackThreads);
+    return;
+  }
+  const uint4* p = reinterpret_cast<const uint4*>(x + cut.head);
+  const int first = part * kPart + threadIdx.x, end = min(cut.vectors, (part + 1) * kPart);
+  uint4 q[kBackVectors];
+#pragma unroll
+  for (int j = 0; j < kBackVectors; ++j)
+    if (first + j * kBackThreads < end) q[j] = __ldcs(p + first + j * kBackThreads);
+  const float c = inv_t * kLog2e, w = grad_logprob[row] * inv_t;
+  const float2 st = stats[row];
+  const pair_t minus = pair(-st.x, -st.x), cc = pair(c, c), less = pair(-st.y, -st.y), scale = pair(-w, -w);
+  const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
+  const bool alike = cut_alike(x, g);
+  const int at = (int)t - cut.head, holder = at / E;
+  const bool inside = at >= 0 && holder < cut.vectors;
+#pragma unroll
+  for (int j = 0; j < kBackVectors; ++j) {
+    const int v = first + j * kBackThreads;
+    if (v < end) {
+      const bool own = inside && v == holder;
+      const float xt = own ? load1(x + t) : 0.f;   // before it may be overwritten
+      put(g + cut.head + (long long)v * E, Vec<T>::map(q[j], f), alike);
+      if (own) store1(g + t, -expm1f((xt - st.x) * inv_t - st.y * kLn2) * w);
+    }
+  }
+  // the elements in front of the vectors belong to the first part, those behind to the last
+  const int loose = threadIdx.x < 16 ? cut.loose(threadIdx.x, vocab) : -1;
+  if (loose >= 0 && (threadIdx.x < 8 ? part == 0 : last)) {
+    const float xv = load1(x + loose);
+    store1(g + loose, loose == (int)t ? -expm1f((xv - st.x) * inv_t - st.y * kLn2) * w
+                                      : exp2_fast((xv - st.x) * c - st.y) * -w);
   }
 }
 
@@ -134,19 +399,43 @@ int check_grad(const char* who, const void* logits, int dtype, int64_t row_strid
   return fail(MOLT_E_VALUE, "%s: the gradient overlaps the logits without being the same rows", who);
 }
 
+template <typename T, bool GRAD, int THREADS, int NB, int BLOCKS>
+int launch_row_kernel(int cluster, const void* logits, int64_t row_stride, const int64_t* ids, const float* weight,
+                      float temperature, float* logprob, float* stats, void* grad, int64_t grad_stride, int64_t rows,
+                      int64_t vocab, cudaStream_t s) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(rows * cluster));
+  config.blockDim = dim3(THREADS);
+  config.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = cluster > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&config, row_kernel<T, GRAD, THREADS, NB, BLOCKS>, reinterpret_cast<const T*>(logits), (long long)row_stride,
+                     reinterpret_cast<const long long*>(ids), weight, 1.f / temperature, logprob, reinterpret_cast<float2*>(stats),
+                     reinterpret_cast<T*>(grad), (long long)grad_stride, (int)vocab);
+  return launch_status("token_logprob row_kernel");
+}
+
 template <typename T>
 int launch_rows(const void* logits, int64_t row_stride, const int64_t* ids, const float* weight, float temperature,
                 float* logprob, float* stats, void* grad, int64_t grad_stride, int64_t rows, int64_t vocab, cudaStream_t s) {
-  auto* x = reinterpret_cast<const T*>(logits);
-  auto* id = reinterpret_cast<const long long*>(ids);
-  auto* st = reinterpret_cast<float2*>(stats);
-  if (grad != nullptr)
-    row_kernel<T, true><<<(unsigned)rows, kThreads, 0, s>>>(x, row_stride, id, weight, 1.f / temperature, logprob, st,
-                                                            reinterpret_cast<T*>(grad), grad_stride, (int)vocab);
-  else
-    row_kernel<T, false><<<(unsigned)rows, kThreads, 0, s>>>(x, row_stride, id, weight, 1.f / temperature, logprob, st, nullptr, 0,
-                                                             (int)vocab);
-  return launch_status("token_logprob row_kernel");
+  const int64_t vectors = vocab / Vec<T>::kElements;
+#define MOLT_ROWS(GRAD, THREADS, NB, BLOCKS, CLUSTER)                                                                       \
+  launch_row_kernel<T, GRAD, THREADS, NB, BLOCKS>(CLUSTER, logits, row_stride, ids, weight, temperature, logprob, stats, grad, \
+                                                  grad_stride, rows, vocab, s)
+  if (vectors <= 64 * 8) return grad != nullptr ? MOLT_ROWS(true, 64, 2, 16, 1) : MOLT_ROWS(false, 64, 2, 16, 1);
+  int cluster = 1;
+  if (grad != nullptr) {
+    while (cluster < 8 && (vectors > cluster * 256 * 20 || (rows * cluster < 148 * 4 && vectors >= cluster * 256 * 4))) cluster *= 2;
+    return MOLT_ROWS(true, 256, 4, 5, cluster);
+  }
+  while (cluster < 8 && rows * cluster < 148 * 2 && vectors >= cluster * 512 * 4) cluster *= 2;
+  return MOLT_ROWS(false, 512, 4, (sizeof(T) == 2 ? 4 : 3), cluster);
+#undef MOLT_ROWS
 }
 
 }  // namespace
@@ -192,13 +481,18 @@ extern "C" int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto* id = reinterpret_cast<const long long*>(token_ids);
   auto* st = reinterpret_cast<const float2*>(stats);
+  const int64_t per_part = (int64_t)kBackThreads * kBackVectors * (dtype == MOLT_DTYPE_BF16 ? 8 : 4);
+  const int64_t parts = (vocab + per_part - 1) / per_part;
+  MOLT_REQUIRE(rows * parts < (1LL << 31), MOLT_E_CAPABILITY, "%s: more than 2^31 blocks of logits", who);
+  const unsigned blocks = (unsigned)(rows * parts);
   if (dtype == MOLT_DTYPE_BF16)
-    backward_kernel<__nv_bfloat16><<<(unsigned)rows, kThreads, 0, s>>>(
+    backward_kernel<__nv_bfloat16><<<blocks, kBackThreads, 0, s>>>(
         reinterpret_cast<const __nv_bfloat16*>(logits), row_stride, id, st, grad_logprob, 1.f / temperature,
-        reinterpret_cast<__nv_bfloat16*>(grad_logits), grad_stride, (int)vocab);
+        reinterpret_cast<__nv_bfloat16*>(grad_logits), grad_stride, (int)vocab, (int)parts);
   else
-    backward_kernel<float><<<(unsigned)rows, kThreads, 0, s>>>(reinterpret_cast<const float*>(logits), row_stride, id, st,
-                                                               grad_logprob, 1.f / temperature,
-                                                               reinterpret_cast<float*>(grad_logits), grad_stride, (int)vocab);
+    backward_kernel<float><<<blocks, kBackThreads, 0, s>>>(reinterpret_cast<const float*>(logits), row_stride, id, st,
+                                                           grad_logprob, 1.f / temperature,
+                                                           reinterpret_cast<float*>(grad_logits), grad_stride, (int)vocab,
+                                                           (int)parts);
   return launch_status("token_logprob backward_kernel");
 }
