@@ -234,7 +234,8 @@ def check(code: int) -> None:
 
 
 def stream_handle(device: Optional[torch.device] = None) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)   # no Stream object: this stands in front of every call
 
 
 def ptr(tensor: Optional[torch.Tensor]) -> Optional[int]:

@@ -2,8 +2,8 @@
 //   norm = (sum g^2)^(1/2)  or  max |g|;   coefficient = min(1, max_norm / (norm + 1e-6));   out = g * coefficient
 // The list travels in the kernel's parameters (no copy to the device, nothing kept, capture-safe); a list longer than a
 // table is walked in several launches.  Every tensor is cut into chunks, the chunks of the list are numbered through, and
-// block i of G takes chunks i, i + G, ...; it leaves one partial sum, and the partial sums are added in their order, so a list
-// gives the same bits on every call.
+// block i of G takes chunks i, i + G, ...; it leaves one partial sum, and the partial sums are added in a fixed order, so a
+// list gives the same bits on every call.
 #include <math.h>
 
 #include <algorithm>
@@ -15,19 +15,22 @@ namespace molt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTable = 512;          // tensors per launch: the table must stay below the 32764 bytes of kernel parameters
 constexpr int kChunk = 8192;         // elements of a chunk
-constexpr int kBlocks = 148 * 4;     // a fixed figure: it decides which chunks one partial sum holds
+constexpr int kBlocks = 148 * 5;     // a fixed figure: it decides which chunks one partial sum holds
+constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 
+template <int CAPACITY>
 struct Table {
-  const void* grad[kTable];
-  void* out[kTable];
-  long long elements[kTable];
-  unsigned first[kTable + 1];        // number of a tensor's first chunk; [count] = all chunks
-  unsigned char half[kTable];        // bf16
+  const void* grad[CAPACITY];
+  void* out[CAPACITY];
+  long long elements[CAPACITY];
+  unsigned first[CAPACITY + 1];      // number of a tensor's first chunk; [count] = all chunks
+  unsigned char half[CAPACITY];      // bf16
   int count;
 };
-static_assert(sizeof(Table) < 32000, "kernel parameters");
+constexpr int kTable = 1024;         // tensors per launch: the table must stay below the 32764 bytes of kernel parameters
+constexpr int kSmallTable = 16;      // a short list, such as one arena, does not carry 30 KB to the device
+static_assert(sizeof(Table<kTable>) < 32000, "kernel parameters");
 
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -47,14 +50,14 @@ __device__ __forceinline__ double block_total(double v) {
   }
   if (lane == 0) part[warp] = v;
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int w = 1; w < warps; ++w) v = MAX ? larger(v, part[w]) : v + part[w];
-  __syncthreads();
+  v = part[0];
+  for (int w = 1; w < warps; ++w) v = MAX ? larger(v, part[w]) : v + part[w];
   return v;
 }
 
 // The tensor that chunk `c` belongs to.
-__device__ __forceinline__ int tensor_of(const Table& table, unsigned c) {
+template <int CAPACITY>
+__device__ __forceinline__ int tensor_of(const Table<CAPACITY>& table, unsigned c) {
   int low = 0, high = table.count - 1;
   while (low < high) {
     const int middle = (low + high + 1) >> 1;
@@ -64,17 +67,106 @@ __device__ __forceinline__ int tensor_of(const Table& table, unsigned c) {
   return low;
 }
 
+// The elements of 16 bytes.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kElements = 4;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int kElements = 8;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf16_lo(w[i]);
+      v[2 * i + 1] = bf16_hi(w[i]);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+};
+
+// A stretch of elements: those in front of its 16-byte vectors, the vectors, those behind.
+template <typename T>
+struct Cut {
+  int head, vectors, tail;
+  __device__ __forceinline__ Cut(const T* g, int n) {
+    head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / sizeof(T)));
+    vectors = (n - head) / Vec<T>::kElements;
+    tail = n - head - vectors * Vec<T>::kElements;
+  }
+  // The element outside the vectors that this thread looks after, or -1.
+  __device__ __forceinline__ int loose(int n) const {
+    const int i = threadIdx.x;
+    return i < 8 ? (i < head ? i : -1) : (i < 16 && i - 8 < tail ? n - tail + i - 8 : -1);
+  }
+};
+
+// Squares of one vector: in fp32 where neither a square nor their sum leaves its range (the sum of at most 8 is then
+// within 10 roundings), else in 64 bits.  Below 2^-80 a square may have been flushed that is not small beside the others.
+template <int N>
+__device__ __forceinline__ double squares(const float (&v)[N], const uint4& q) {
+  float a = v[0] * v[0], b = v[1] * v[1];
+#pragma unroll
+  for (int i = 2; i < N; i += 2) {
+    a = fmaf(v[i], v[i], a);
+    b = fmaf(v[i + 1], v[i + 1], b);
+  }
+  const float sum = a + b;
+  if (sum >= 0x1p-80f && sum <= 0x1.fffffep127f) return sum;
+  if ((q.x | q.y | q.z | q.w) == 0u) return 0.;
+  double exact = 0.;
+#pragma unroll
+  for (int i = 0; i < N; ++i) exact += (double)v[i] * (double)v[i];
+  return exact;
+}
+
+template <int N>
+__device__ __forceinline__ float magnitude(const float (&v)[N]) {   // NaN if there is one
+  float top = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[i])));
+  return top;
+}
+
 template <bool MAX, typename T>
 __device__ __forceinline__ double chunk_total(const T* g, int n, double acc) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const double v = load1(g + i);
-    acc = MAX ? larger(acc, fabs(v)) : acc + v * v;
+  constexpr int E = Vec<T>::kElements;
+  const Cut<T> cut(g, n);
+  const uint4* p = reinterpret_cast<const uint4*>(g + cut.head);
+  for (int v = threadIdx.x; v < cut.vectors; v += kUnroll * kThreads) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) q[j] = v + j * kThreads < cut.vectors ? p[v + j * kThreads] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      float x[E];
+      Vec<T>::unpack(q[j], x);
+      if (MAX) acc = larger(acc, (double)magnitude(x));
+      else acc += squares(x, q[j]);
+    }
+  }
+  const int own = cut.loose(n);
+  if (own >= 0) {
+    const double x = load1(g + own);
+    acc = MAX ? larger(acc, fabs(x)) : acc + x * x;
   }
   return acc;
 }
 
-template <bool MAX>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table table, double* __restrict__ part) {
+template <bool MAX, int CAPACITY>
+__global__ void __launch_bounds__(kThreads, 5) norm_kernel(const __grid_constant__ Table<CAPACITY> table,
+                                                        double* __restrict__ part) {
   double acc = 0.;
   const unsigned chunks = table.first[table.count];
   for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -88,45 +180,88 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
+// The norm and the coefficient from the partial sums, by one block; every thread gets them.
 template <bool MAX>
-__global__ void __launch_bounds__(1024) norm_finish_kernel(const double* __restrict__ part, int parts, float grad_scale,
-                                                           float max_norm, float* __restrict__ result) {
+__device__ __forceinline__ float2 finish(const double* __restrict__ part, int parts, float grad_scale, float max_norm) {
   double acc = 0.;
   for (int i = threadIdx.x; i < parts; i += blockDim.x) acc = MAX ? larger(acc, part[i]) : acc + part[i];
   acc = block_total<MAX>(acc);
+  const float norm = (float)((MAX ? acc : sqrt(acc)) * fabs((double)grad_scale));
+  const float c = max_norm / (norm + 1e-6f);
+  return make_float2(norm, c > 1.f ? 1.f : c);   // NaN stays
+}
+
+template <bool MAX>
+__global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* __restrict__ part, int parts, float grad_scale,
+                                                               float max_norm, float* __restrict__ result) {
+  const float2 r = finish<MAX>(part, parts, grad_scale, max_norm);
   if (threadIdx.x == 0) {
-    const float norm = (float)((MAX ? acc : sqrt(acc)) * fabs((double)grad_scale));
-    const float c = max_norm / (norm + 1e-6f);
-    result[0] = norm;
-    result[1] = c > 1.f ? 1.f : c;   // NaN stays
+    result[0] = r.x;
+    result[1] = r.y;
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const T* g, T* out, int n, float c) {
-  for (int i = threadIdx.x; i < n; i += kThreads) store1(out + i, load1(g + i) * c);
+  constexpr int E = Vec<T>::kElements;
+  const Cut<T> cut(g, n);
+  const uint4* p = reinterpret_cast<const uint4*>(g + cut.head);
+  T* to = out + cut.head;
+  const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  for (int v = threadIdx.x; v < cut.vectors; v += kUnroll * kThreads) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j)
+      if (v + j * kThreads < cut.vectors) q[j] = __ldcs(p + v + j * kThreads);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      if (v + j * kThreads >= cut.vectors) continue;
+      float x[E];
+      Vec<T>::unpack(q[j], x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] *= c;
+      if (alike) {
+        __stcs(reinterpret_cast<uint4*>(to) + v + j * kThreads, Vec<T>::pack(x));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) store1(to + (v + j * kThreads) * E + i, x[i]);
+      }
+    }
+  }
+  const int own = cut.loose(n);
+  if (own >= 0) store1(out + own, load1(g + own) * c);
 }
 
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table table, const float* __restrict__ result) {
-  const float coefficient = result[1];
+// Every block adds the partial sums up for itself (they lie in the L2) instead of waiting for one that does.  The chunks
+// are taken from the last to the first: what the norm read last is what the L2 still holds.
+template <bool MAX, int CAPACITY>
+__global__ void __launch_bounds__(kThreads, 6) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
+                                                         const double* __restrict__ part, int parts, float max_norm,
+                                                         float* __restrict__ result) {
+  const float2 r = finish<MAX>(part, parts, 1.f, max_norm);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    result[0] = r.x;
+    result[1] = r.y;
+  }
   const unsigned chunks = table.first[table.count];
-  for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
+  for (unsigned i = blockIdx.x; i < chunks; i += gridDim.x) {
+    const unsigned c = chunks - 1 - i;
     const int k = tensor_of(table, c);
     const long long begin = (long long)(c - table.first[k]) * kChunk;
     const int n = (int)min((long long)kChunk, table.elements[k] - begin);
     if (table.half[k])
       chunk_scale(reinterpret_cast<const __nv_bfloat16*>(table.grad[k]) + begin,
-                  reinterpret_cast<__nv_bfloat16*>(table.out[k]) + begin, n, coefficient);
+                  reinterpret_cast<__nv_bfloat16*>(table.out[k]) + begin, n, r.y);
     else
-      chunk_scale(reinterpret_cast<const float*>(table.grad[k]) + begin, reinterpret_cast<float*>(table.out[k]) + begin, n,
-                  coefficient);
+      chunk_scale(reinterpret_cast<const float*>(table.grad[k]) + begin, reinterpret_cast<float*>(table.out[k]) + begin, n, r.y);
   }
 }
 
 int tables_of(int count) { return (count + kTable - 1) / kTable; }
 
 // Fills `table` with items [begin, begin + n).
-void fill(Table& table, const molt_grad_item* items, int n) {
+template <int CAPACITY>
+void fill(Table<CAPACITY>& table, const molt_grad_item* items, int n) {
   table.count = n;
   unsigned chunks = 0;
   for (int k = 0; k < n; ++k) {
@@ -138,6 +273,35 @@ void fill(Table& table, const molt_grad_item* items, int n) {
     chunks += (unsigned)((items[k].count + kChunk - 1) / kChunk);
   }
   table.first[n] = chunks;
+}
+
+template <bool MAX>
+int launch_norm(const molt_grad_item* items, int n, double* part, cudaStream_t s) {
+  if (n <= kSmallTable) {
+    Table<kSmallTable> table;
+    fill(table, items, n);
+    norm_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part);
+  } else {
+    Table<kTable> table;
+    fill(table, items, n);
+    norm_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part);
+  }
+  return launch_status("norm_kernel");
+}
+
+template <bool MAX>
+int launch_scale(const molt_grad_item* items, int n, const double* part, int parts, float max_norm, float* result,
+                 cudaStream_t s) {
+  if (n <= kSmallTable) {
+    Table<kSmallTable> table;
+    fill(table, items, n);
+    scale_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+  } else {
+    Table<kTable> table;
+    fill(table, items, n);
+    scale_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+  }
+  return launch_status("scale_kernel");
 }
 
 struct Span {
@@ -200,22 +364,24 @@ int norm_launch(const char* who, const molt_grad_item* items, int count, int nor
   if (clip)
     if (int rc = check_overlap(who, items, count)) return rc;
   auto* part = reinterpret_cast<double*>(workspace);
-  Table table;
-  for (int t = 0; t < tables_of(count); ++t) {
-    fill(table, items + t * kTable, std::min(kTable, count - t * kTable));
-    if (norm_kind == MOLT_NORM_MAX) norm_kernel<true><<<kBlocks, kThreads, 0, s>>>(table, part + t * kBlocks);
-    else norm_kernel<false><<<kBlocks, kThreads, 0, s>>>(table, part + t * kBlocks);
-    if (int rc = launch_status("norm_kernel")) return rc;
-  }
   const int parts = tables_of(count) * kBlocks;
-  if (norm_kind == MOLT_NORM_MAX) norm_finish_kernel<true><<<1, 1024, 0, s>>>(part, parts, grad_scale, max_norm, result);
-  else norm_finish_kernel<false><<<1, 1024, 0, s>>>(part, parts, grad_scale, max_norm, result);
-  if (int rc = launch_status("norm_finish_kernel")) return rc;
-  if (!clip) return MOLT_OK;
+  const bool max = norm_kind == MOLT_NORM_MAX;
   for (int t = 0; t < tables_of(count); ++t) {
-    fill(table, items + t * kTable, std::min(kTable, count - t * kTable));
-    scale_kernel<<<kBlocks, kThreads, 0, s>>>(table, result);
-    if (int rc = launch_status("scale_kernel")) return rc;
+    const int n = std::min(kTable, count - t * kTable);
+    if (int rc = max ? launch_norm<true>(items + t * kTable, n, part + t * kBlocks, s)
+                     : launch_norm<false>(items + t * kTable, n, part + t * kBlocks, s))
+      return rc;
+  }
+  if (!clip) {
+    if (max) norm_finish_kernel<true><<<1, kThreads, 0, s>>>(part, parts, grad_scale, max_norm, result);
+    else norm_finish_kernel<false><<<1, kThreads, 0, s>>>(part, parts, grad_scale, max_norm, result);
+    return launch_status("norm_finish_kernel");
+  }
+  for (int t = tables_of(count) - 1; t >= 0; --t) {
+    const int n = std::min(kTable, count - t * kTable);
+    if (int rc = max ? launch_scale<true>(items + t * kTable, n, part, parts, max_norm, result, s)
+                     : launch_scale<false>(items + t * kTable, n, part, parts, max_norm, result, s))
+      return rc;
   }
   return MOLT_OK;
 }

@@ -37,22 +37,26 @@ def _stride(rows: torch.Tensor) -> int:
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
+def _forward(rows: torch.Tensor, ids: torch.Tensor, temperature: float, stats: Optional[torch.Tensor]) -> torch.Tensor:
+    device = rows.device
+    logprobs = torch.empty(ids.shape, dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        _native.check(_native.library().molt_token_logprob_fwd(
+            rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), temperature, logprobs.data_ptr(),
+            _native.ptr(stats), rows.shape[0], rows.shape[1], _native.stream_handle(device)))
+    return logprobs
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """Saves the logits (by reference), the ids and two floats per row."""
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, token_ids: torch.Tensor, temperature: float) -> torch.Tensor:
         rows, ids = _rows(logits), token_ids.contiguous()
-        logprobs = torch.empty(token_ids.shape, dtype=torch.float32, device=logits.device)
-        stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=logits.device) if ctx.needs_input_grad[0] else None
-        with torch.cuda.device(logits.device):
-            _native.check(_native.library().molt_token_logprob_fwd(
-                rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), temperature, logprobs.data_ptr(),
-                _native.ptr(stats), rows.shape[0], rows.shape[1], _native.stream_handle(logits.device)))
-        if stats is not None:
-            ctx.save_for_backward(rows, ids, stats)
-            ctx.shape, ctx.temperature = logits.shape, temperature
-        return logprobs
+        stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=rows.device)
+        ctx.save_for_backward(rows, ids, stats)
+        ctx.shape, ctx.temperature = logits.shape, temperature
+        return _forward(rows, ids, temperature, stats)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -75,7 +79,9 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, temperature: f
     outside ``[0, vocab)`` (an ignore index such as -100) gives 0 and no gradient, whatever its row holds.  Logits of -inf
     have probability zero; a row without a finite logit, or with a NaN or +inf, gives NaN."""
     _check(logits, token_ids)
-    return _TokenLogprobs.apply(logits, token_ids, float(temperature))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogprobs.apply(logits, token_ids, float(temperature))
+    return _forward(_rows(logits), token_ids.contiguous(), float(temperature), None)
 
 
 @torch.no_grad()
