@@ -351,7 +351,7 @@ int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, c
  * row_strides: elements between the rows of logprob, old, ref, advantage (between its entries when it is [batch]), mask.
  * loss[0]; stats[2] = mean k, mean of 1[the clamp cut the gradient].  For the backward (unit_grad NULL: not wanted):
  * unit_grad [batch, seq] receives d l / d logprob per token, zero behind the mask, and row_weight [batch] the weight of
- * a kept token of the row.  The clamp's border is decided in 64 bits, sums are kept in 64 bits, in a fixed order. */
+ * a kept token of the row.  A small batch needs no workspace (0 bytes, NULL).  The clamp's border is decided in 64 bits, sums are kept in 64 bits, in a fixed order. */
 size_t molt_policy_loss_workspace_bytes(int64_t batch, int64_t seq);
 int molt_policy_loss_fwd(const float* logprob, const float* old_logprob, const float* ref_logprob, const float* advantage,
                          int advantage_per_token, const uint8_t* mask, const int64_t row_strides[5], int64_t batch,
@@ -370,7 +370,7 @@ int molt_policy_loss_bwd(const float* unit_grad, const float* row_weight, const 
  * h[p] = s[p] - s[pairs + p], loss[0] = mean over pairs.  ref_logprob: NULL (0), or with ref_per_token != 0 [2 * pairs, seq],
  * else [2 * pairs] values subtracted from the rows' sums (their means).  row_strides: of logprob, ref (between entries
  * when it is [2 * pairs]), mask.  rewards[2 * pairs] = beta * s.  seq_grad[2 * pairs] = d loss / d (a kept token of the row).
- * Sums are kept in 64 bits, in a fixed order. */
+ * A small batch needs no workspace (0 bytes, NULL).  Sums are kept in 64 bits, in a fixed order. */
 size_t molt_preference_loss_workspace_bytes(int64_t pairs, int64_t seq);
 int molt_preference_loss_fwd(const float* logprob, const float* ref_logprob, int ref_per_token, const uint8_t* mask,
                              const int64_t row_strides[3], int64_t pairs, int64_t seq, double beta, double smoothing, int kind,

@@ -16,7 +16,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;         // elements of a chunk
-constexpr int kBlocks = 148 * 5;     // a fixed figure: it decides which chunks one partial sum holds
+constexpr int kBlocks = 148 * 5;     // most partial sums of one table; a fixed figure, it decides which chunks one of them holds
+constexpr int kScaleBlocks = 148 * 32;   // many more than run at a time: blocks that begin late even out the others
 constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 
 template <int CAPACITY>
@@ -206,27 +207,24 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int n, float c) 
   constexpr int E = Vec<T>::kElements;
   const Cut<T> cut(g, n);
   const uint4* p = reinterpret_cast<const uint4*>(g + cut.head);
-  T* to = out + cut.head;
-  const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  for (int v = threadIdx.x; v < cut.vectors; v += kUnroll * kThreads) {
-    uint4 q[kUnroll];
+  if (((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+    uint4* to = reinterpret_cast<uint4*>(out + cut.head);
+    for (int v = threadIdx.x; v < cut.vectors; v += kUnroll * kThreads) {
+      uint4 q[kUnroll];
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j)
-      if (v + j * kThreads < cut.vectors) q[j] = __ldcs(p + v + j * kThreads);
+      for (int j = 0; j < kUnroll; ++j)
+        if (v + j * kThreads < cut.vectors) q[j] = __ldcs(p + v + j * kThreads);
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      if (v + j * kThreads >= cut.vectors) continue;
-      float x[E];
-      Vec<T>::unpack(q[j], x);
+      for (int j = 0; j < kUnroll; ++j) {
+        float x[E];
+        Vec<T>::unpack(q[j], x);
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] *= c;
-      if (alike) {
-        __stcs(reinterpret_cast<uint4*>(to) + v + j * kThreads, Vec<T>::pack(x));
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) store1(to + (v + j * kThreads) * E + i, x[i]);
+        for (int i = 0; i < E; ++i) x[i] *= c;
+        if (v + j * kThreads < cut.vectors) __stcs(to + v + j * kThreads, Vec<T>::pack(x));
       }
     }
+  } else {   // an output cut elsewhere than its gradient: element by element
+    for (int i = cut.head + threadIdx.x; i < n - cut.tail; i += kThreads) store1(out + i, load1(g + i) * c);
   }
   const int own = cut.loose(n);
   if (own >= 0) store1(out + own, load1(g + own) * c);
@@ -235,7 +233,7 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int n, float c) 
 // Every block adds the partial sums up for itself (they lie in the L2) instead of waiting for one that does.  The chunks
 // are taken from the last to the first: what the norm read last is what the L2 still holds.
 template <bool MAX, int CAPACITY>
-__global__ void __launch_bounds__(kThreads, 6) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
+__global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
                                                          const double* __restrict__ part, int parts, float max_norm,
                                                          float* __restrict__ result) {
   const float2 r = finish<MAX>(part, parts, 1.f, max_norm);
@@ -276,32 +274,39 @@ void fill(Table<CAPACITY>& table, const molt_grad_item* items, int n) {
 }
 
 template <bool MAX>
-int launch_norm(const molt_grad_item* items, int n, double* part, cudaStream_t s) {
+int launch_norm(const molt_grad_item* items, int n, int blocks, double* part, cudaStream_t s) {
   if (n <= kSmallTable) {
     Table<kSmallTable> table;
     fill(table, items, n);
-    norm_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part);
+    norm_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part);
   } else {
     Table<kTable> table;
     fill(table, items, n);
-    norm_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part);
+    norm_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part);
   }
   return launch_status("norm_kernel");
 }
 
 template <bool MAX>
-int launch_scale(const molt_grad_item* items, int n, const double* part, int parts, float max_norm, float* result,
+int launch_scale(const molt_grad_item* items, int n, int blocks, const double* part, int parts, float max_norm, float* result,
                  cudaStream_t s) {
   if (n <= kSmallTable) {
     Table<kSmallTable> table;
     fill(table, items, n);
-    scale_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+    scale_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
   } else {
     Table<kTable> table;
     fill(table, items, n);
-    scale_kernel<MAX><<<kBlocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+    scale_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
   }
   return launch_status("scale_kernel");
+}
+
+// Blocks for the chunks of a table, at least one.
+int blocks_for(const molt_grad_item* items, int n, int most) {
+  long long chunks = 0;
+  for (int k = 0; k < n; ++k) chunks += (items[k].count + kChunk - 1) / kChunk;
+  return (int)std::max(1LL, std::min((long long)most, chunks));
 }
 
 struct Span {
@@ -364,13 +369,14 @@ int norm_launch(const char* who, const molt_grad_item* items, int count, int nor
   if (clip)
     if (int rc = check_overlap(who, items, count)) return rc;
   auto* part = reinterpret_cast<double*>(workspace);
-  const int parts = tables_of(count) * kBlocks;
   const bool max = norm_kind == MOLT_NORM_MAX;
+  int parts = 0;
   for (int t = 0; t < tables_of(count); ++t) {
-    const int n = std::min(kTable, count - t * kTable);
-    if (int rc = max ? launch_norm<true>(items + t * kTable, n, part + t * kBlocks, s)
-                     : launch_norm<false>(items + t * kTable, n, part + t * kBlocks, s))
+    const molt_grad_item* first = items + t * kTable;
+    const int n = std::min(kTable, count - t * kTable), blocks = blocks_for(first, n, kBlocks);
+    if (int rc = max ? launch_norm<true>(first, n, blocks, part + parts, s) : launch_norm<false>(first, n, blocks, part + parts, s))
       return rc;
+    parts += blocks;
   }
   if (!clip) {
     if (max) norm_finish_kernel<true><<<1, kThreads, 0, s>>>(part, parts, grad_scale, max_norm, result);
@@ -378,9 +384,10 @@ int norm_launch(const char* who, const molt_grad_item* items, int count, int nor
     return launch_status("norm_finish_kernel");
   }
   for (int t = tables_of(count) - 1; t >= 0; --t) {
-    const int n = std::min(kTable, count - t * kTable);
-    if (int rc = max ? launch_scale<true>(items + t * kTable, n, part, parts, max_norm, result, s)
-                     : launch_scale<false>(items + t * kTable, n, part, parts, max_norm, result, s))
+    const molt_grad_item* first = items + t * kTable;
+    const int n = std::min(kTable, count - t * kTable), blocks = blocks_for(first, n, kScaleBlocks);
+    if (int rc = max ? launch_scale<true>(first, n, blocks, part, parts, max_norm, result, s)
+                     : launch_scale<false>(first, n, blocks, part, parts, max_norm, result, s))
       return rc;
   }
   return MOLT_OK;

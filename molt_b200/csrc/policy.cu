@@ -40,6 +40,13 @@ int splits_for(int64_t rows, int64_t seq) {
   return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
 }
 
+// A batch this small is one block's work: its row sums stay in shared memory and one launch gives the loss (4 x 64 tokens,
+// whole call with its backward: 135 us of host time with two launches and a workspace, 113 us with one).
+constexpr int kOneBlock = 1024, kOneBlockRows = 256, kOneBlockTokens = 8192;
+bool one_block(int64_t rows, int64_t seq) { return rows <= kOneBlockRows && rows * seq <= kOneBlockTokens; }
+// Warps of the one block that share a row.
+int one_block_splits(int64_t rows) { return rows >= kOneBlock / 32 ? 1 : (int)(kOneBlock / 32 / rows); }
+
 // ---- clipped policy loss -------------------------------------------------------------------------------------------
 struct PolicyArgs {
   const float *logprob, *old, *ref, *advantage;
@@ -62,47 +69,57 @@ __device__ __forceinline__ float exp_minus_1_minus(float d) {
   return 0.5f * d * d * r;
 }
 
-__global__ void __launch_bounds__(kThreads) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad, double* __restrict__ part) {
-  const long long b = blockIdx.x;
-  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
-  double sum[4] = {0., 0., 0., 0.};   // loss, k, cut, kept
-  for (long long t = begin + threadIdx.x; t < end; t += kThreads) {
-    float g = 0.f;
-    if (a.mask == nullptr || a.mask[b * a.mask_stride + t] != 0) {
-      const float lp = a.logprob[b * a.lp_stride + t];
-      const float old = a.old[b * a.old_stride + t];
-      const float adv = a.advantage[b * a.adv_stride + (a.per_token ? t : 0)];
-      const double d = (double)lp - (double)old;
-      const bool cut = (adv > 0.f && d > a.log_high) || (adv < 0.f && d < a.log_low);
-      float l = 0.f;
-      if (adv != 0.f) {   // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
-        const float r = expf((float)d);
-        l = -(cut ? (adv > 0.f ? a.high : a.low) : r) * adv;
-        g = cut ? 0.f : -r * adv;
+// Tokens begin, begin + step, ... below end of row b, kUnroll of them loaded at a time.
+constexpr int kUnroll = 4;
+
+__device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, long long begin, long long end, int step,
+                                              float* __restrict__ unit_grad, double (&sum)[4]) {
+  for (long long t0 = begin; t0 < end; t0 += kUnroll * step) {
+    float lp[kUnroll], old[kUnroll], adv[kUnroll], ref[kUnroll];
+    bool kept[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long t = t0 + j * step;
+      kept[j] = t < end;
+      if (kept[j]) {
+        lp[j] = a.logprob[b * a.lp_stride + t];
+        old[j] = a.old[b * a.old_stride + t];
+        adv[j] = a.advantage[b * a.adv_stride + (a.per_token ? t : 0)];
+        ref[j] = a.ref != nullptr ? a.ref[b * a.ref_stride + t] : 0.f;
+        kept[j] = a.mask == nullptr || a.mask[b * a.mask_stride + t] != 0;
       }
-      float k = 0.f;
-      if (a.ref != nullptr) {
-        const float e = a.ref[b * a.ref_stride + t] - lp;
-        k = exp_minus_1_minus(e);
-        l += a.kl_coef * k;
-        g -= a.kl_coef * expm1f(e);
-      }
-      sum[0] += l;
-      sum[1] += k;
-      sum[2] += cut ? 1. : 0.;
-      sum[3] += 1.;
     }
-    if (unit_grad != nullptr) unit_grad[b * a.seq + t] = g;
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      float g = 0.f;
+      if (kept[j]) {
+        const double d = (double)lp[j] - (double)old[j];
+        const bool cut = (adv[j] > 0.f && d > a.log_high) || (adv[j] < 0.f && d < a.log_low);
+        float l = 0.f;
+        if (adv[j] != 0.f) {   // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
+          const float r = expf((float)d);
+          l = -(cut ? (adv[j] > 0.f ? a.high : a.low) : r) * adv[j];
+          g = cut ? 0.f : -r * adv[j];
+        }
+        if (a.ref != nullptr) {
+          const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
+          l += a.kl_coef * k;
+          g -= a.kl_coef * expm1f(e);
+          sum[1] += k;
+        }
+        sum[0] += l;
+        sum[2] += cut ? 1. : 0.;
+        sum[3] += 1.;
+      }
+      if (unit_grad != nullptr && t0 + j * step < end) unit_grad[b * a.seq + t0 + j * step] = g;
+    }
   }
-  block_sum(sum);
-  if (threadIdx.x == 0)
-    for (int i = 0; i < 4; ++i) part[(b * a.splits + blockIdx.y) * 4 + i] = sum[i];
 }
 
-// Row sums, weights and the result, in one block.
-__global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
-                                                             int reduction, float* __restrict__ row_weight,
-                                                             float* __restrict__ loss, float* __restrict__ stats) {
+// Row sums (loss, k, cut, kept), weights and the result, by one block.
+__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction,
+                                              float* __restrict__ row_weight, float* __restrict__ loss,
+                                              float* __restrict__ stats) {
   __shared__ double total;
   double count[1] = {0.};
   for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
@@ -133,6 +150,42 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __res
   }
 }
 
+__global__ void __launch_bounds__(kThreads) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad, double* __restrict__ part) {
+  const long long b = blockIdx.x;
+  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
+  double sum[4] = {0., 0., 0., 0.};
+  policy_tokens(a, b, begin + threadIdx.x, end, kThreads, unit_grad, sum);
+  block_sum(sum);
+  if (threadIdx.x == 0)
+    for (int i = 0; i < 4; ++i) part[(b * a.splits + blockIdx.y) * 4 + i] = sum[i];
+}
+
+__global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
+                                                             int reduction, float* __restrict__ row_weight,
+                                                             float* __restrict__ loss, float* __restrict__ stats) {
+  policy_finish(part, batch, splits, reduction, row_weight, loss, stats);
+}
+
+// The whole forward in one block: a warp takes one of the splits of a row.
+__global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs a, int reduction, float* __restrict__ unit_grad,
+                                                                     float* __restrict__ row_weight, float* __restrict__ loss,
+                                                                     float* __restrict__ stats) {
+  __shared__ double part[kOneBlockRows * 4];
+  const int lane = threadIdx.x & 31, units = (int)a.batch * a.splits;
+  for (int u = threadIdx.x >> 5; u < units; u += kOneBlock / 32) {
+    const int b = u / a.splits, s = u - b * a.splits;
+    double sum[4] = {0., 0., 0., 0.};
+    policy_tokens(a, b, a.seq * s / a.splits + lane, a.seq * (s + 1) / a.splits, 32, unit_grad, sum);
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(~0u, sum[i], o);
+      if (lane == 0) part[u * 4 + i] = sum[i];
+    }
+  }
+  __syncthreads();
+  policy_finish(part, a.batch, a.splits, reduction, row_weight, loss, stats);
+}
+
 __global__ void __launch_bounds__(kThreads) policy_backward_kernel(const float* __restrict__ unit_grad,
                                                                    const float* __restrict__ row_weight,
                                                                    const float* __restrict__ grad_loss,
@@ -140,6 +193,7 @@ __global__ void __launch_bounds__(kThreads) policy_backward_kernel(const float* 
   const long long b = blockIdx.x;
   const long long begin = seq * blockIdx.y / splits, end = seq * (blockIdx.y + 1) / splits;
   const float w = row_weight[b] * grad_loss[0];
+#pragma unroll 4
   for (long long t = begin + threadIdx.x; t < end; t += kThreads) {
     const float u = unit_grad[b * seq + t];
     grad_logprob[b * seq + t] = u == 0.f ? 0.f : u * w;
@@ -156,27 +210,32 @@ struct PreferenceArgs {
   double beta, smoothing;
 };
 
-__global__ void __launch_bounds__(kThreads) preference_kernel(PreferenceArgs a, double* __restrict__ part) {
-  const long long i = blockIdx.x;
-  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
-  double sum[2] = {0., 0.};
-  for (long long t = begin + threadIdx.x; t < end; t += kThreads) {
-    if (a.mask != nullptr && a.mask[i * a.mask_stride + t] == 0) continue;
-    double v = a.logprob[i * a.lp_stride + t];
-    if (a.ref != nullptr && a.ref_per_token) v -= (double)a.ref[i * a.ref_stride + t];
-    sum[0] += v;
-    sum[1] += 1.;
-  }
-  block_sum(sum);
-  if (threadIdx.x == 0) {
-    part[(i * a.splits + blockIdx.y) * 2] = sum[0];
-    part[(i * a.splits + blockIdx.y) * 2 + 1] = sum[1];
+__device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long long i, long long begin, long long end, int step,
+                                                  double (&sum)[2]) {
+  for (long long t0 = begin; t0 < end; t0 += kUnroll * step) {
+    float lp[kUnroll], ref[kUnroll];
+    bool kept[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long t = t0 + j * step;
+      kept[j] = t < end;
+      if (kept[j]) {
+        lp[j] = a.logprob[i * a.lp_stride + t];
+        ref[j] = a.ref != nullptr && a.ref_per_token ? a.ref[i * a.ref_stride + t] : 0.f;
+        kept[j] = a.mask == nullptr || a.mask[i * a.mask_stride + t] != 0;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j)
+      if (kept[j]) {
+        sum[0] += (double)lp[j] - (double)ref[j];
+        sum[1] += 1.;
+      }
   }
 }
 
-__global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
-                                                                 float* __restrict__ seq_grad, float* __restrict__ rewards,
-                                                                 float* __restrict__ loss_out) {
+__device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const double* part, float* __restrict__ seq_grad,
+                                                  float* __restrict__ rewards, float* __restrict__ loss_out) {
   double total[1] = {0.};
   for (long long p = threadIdx.x; p < a.pairs; p += blockDim.x) {
     double s[2], scale[2];
@@ -219,6 +278,42 @@ __global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs 
   if (threadIdx.x == 0) loss_out[0] = (float)total[0];
 }
 
+__global__ void __launch_bounds__(kThreads) preference_kernel(PreferenceArgs a, double* __restrict__ part) {
+  const long long i = blockIdx.x;
+  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
+  double sum[2] = {0., 0.};
+  preference_tokens(a, i, begin + threadIdx.x, end, kThreads, sum);
+  block_sum(sum);
+  if (threadIdx.x == 0) {
+    part[(i * a.splits + blockIdx.y) * 2] = sum[0];
+    part[(i * a.splits + blockIdx.y) * 2 + 1] = sum[1];
+  }
+}
+
+__global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
+                                                                 float* __restrict__ seq_grad, float* __restrict__ rewards,
+                                                                 float* __restrict__ loss) {
+  preference_finish(a, part, seq_grad, rewards, loss);
+}
+
+__global__ void __launch_bounds__(kOneBlock) preference_one_block_kernel(PreferenceArgs a, float* __restrict__ seq_grad,
+                                                                         float* __restrict__ rewards, float* __restrict__ loss) {
+  __shared__ double part[kOneBlockRows * 2];
+  const int lane = threadIdx.x & 31, units = (int)(2 * a.pairs) * a.splits;
+  for (int u = threadIdx.x >> 5; u < units; u += kOneBlock / 32) {
+    const int i = u / a.splits, s = u - i * a.splits;
+    double sum[2] = {0., 0.};
+    preference_tokens(a, i, a.seq * s / a.splits + lane, a.seq * (s + 1) / a.splits, 32, sum);
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(~0u, sum[k], o);
+      if (lane == 0) part[u * 2 + k] = sum[k];
+    }
+  }
+  __syncthreads();
+  preference_finish(a, part, seq_grad, rewards, loss);
+}
+
 __global__ void __launch_bounds__(kThreads) preference_backward_kernel(const uint8_t* __restrict__ mask, long long mask_stride,
                                                                        const float* __restrict__ seq_grad,
                                                                        const float* __restrict__ grad_loss,
@@ -226,6 +321,7 @@ __global__ void __launch_bounds__(kThreads) preference_backward_kernel(const uin
   const long long i = blockIdx.x;
   const long long begin = seq * blockIdx.y / splits, end = seq * (blockIdx.y + 1) / splits;
   const float g = seq_grad[i] * grad_loss[0];
+#pragma unroll 4
   for (long long t = begin + threadIdx.x; t < end; t += kThreads)
     grad_logprob[i * seq + t] = mask == nullptr || mask[i * mask_stride + t] != 0 ? g : 0.f;
 }
@@ -247,7 +343,7 @@ int check_stride(const char* who, const char* what, int64_t stride, int64_t leas
 using namespace molt;
 
 extern "C" size_t molt_policy_loss_workspace_bytes(int64_t batch, int64_t seq) {
-  if (batch <= 0 || seq < 0) return 0;
+  if (batch <= 0 || seq < 0 || one_block(batch, seq)) return 0;
   return (size_t)batch * splits_for(batch, seq) * 4 * sizeof(double);
 }
 
@@ -263,12 +359,13 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
                reduction);
   MOLT_REQUIRE(clip_low >= 0. && clip_low <= 1. && clip_high >= 0. && isfinite(clip_high) && isfinite(kl_coef), MOLT_E_VALUE,
                "%s: clip_low must lie in [0, 1], clip_high and kl_coef must be finite, clip_high not negative", who);
-  MOLT_REQUIRE(row_strides && loss && stats && workspace &&
+  MOLT_REQUIRE(row_strides && loss && stats &&
                    (seq == 0 || (unit_grad == nullptr) == (row_weight == nullptr)),
                MOLT_E_VALUE, "%s: NULL pointer", who);
   MOLT_REQUIRE(seq == 0 || (logprob && old_logprob && advantage), MOLT_E_VALUE, "%s: NULL tensor pointer", who);
-  MOLT_REQUIRE(workspace_bytes >= molt_policy_loss_workspace_bytes(batch, seq) && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
-               MOLT_E_VALUE, "%s: the workspace is too small or not 8-byte aligned", who);
+  const size_t needed = molt_policy_loss_workspace_bytes(batch, seq);
+  MOLT_REQUIRE(needed == 0 || (workspace && workspace_bytes >= needed && reinterpret_cast<uintptr_t>(workspace) % 8 == 0), MOLT_E_VALUE,
+               "%s: the workspace is too small or not 8-byte aligned", who);
   const char* names[5] = {"logprob", "old_logprob", "ref_logprob", "advantage", "mask"};
   for (int i = 0; i < 5; ++i)
     if (int rc = check_stride(who, names[i], row_strides[i], i == 3 && !advantage_per_token ? 1 : seq)) return rc;
@@ -280,6 +377,11 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
   a.log_high = log1p(clip_high); a.log_low = log1p(-clip_low);
   a.high = (float)(1. + clip_high); a.low = (float)(1. - clip_low); a.kl_coef = (float)kl_coef;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (needed == 0) {
+    a.splits = one_block_splits(batch);
+    policy_one_block_kernel<<<1, kOneBlock, 0, s>>>(a, reduction, unit_grad, row_weight, loss, stats);
+    return launch_status("policy_one_block_kernel");
+  }
   auto* part = reinterpret_cast<double*>(workspace);
   policy_kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
   if (int rc = launch_status("policy_kernel")) return rc;
@@ -300,7 +402,7 @@ extern "C" int molt_policy_loss_bwd(const float* unit_grad, const float* row_wei
 }
 
 extern "C" size_t molt_preference_loss_workspace_bytes(int64_t pairs, int64_t seq) {
-  if (pairs <= 0 || seq < 0) return 0;
+  if (pairs <= 0 || seq < 0 || one_block(2 * pairs, seq)) return 0;
   return (size_t)pairs * 2 * splits_for(pairs * 2, seq) * 2 * sizeof(double);
 }
 
@@ -315,9 +417,10 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
   MOLT_REQUIRE(beta > 0. && isfinite(beta) && smoothing >= 0. && smoothing <= 1., MOLT_E_VALUE,
                "%s: beta must be positive and finite, the smoothing in [0, 1]", who);
   MOLT_REQUIRE(smoothing == 0. || kind == MOLT_PREFERENCE_SIGMOID, MOLT_E_VALUE, "%s: only the sigmoid loss has label smoothing", who);
-  MOLT_REQUIRE(row_strides && rewards && loss && workspace && (seq == 0 || logprob), MOLT_E_VALUE, "%s: NULL pointer", who);
-  MOLT_REQUIRE(workspace_bytes >= molt_preference_loss_workspace_bytes(pairs, seq) && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
-               MOLT_E_VALUE, "%s: the workspace is too small or not 8-byte aligned", who);
+  MOLT_REQUIRE(row_strides && rewards && loss && (seq == 0 || logprob), MOLT_E_VALUE, "%s: NULL pointer", who);
+  const size_t needed = molt_preference_loss_workspace_bytes(pairs, seq);
+  MOLT_REQUIRE(needed == 0 || (workspace && workspace_bytes >= needed && reinterpret_cast<uintptr_t>(workspace) % 8 == 0), MOLT_E_VALUE,
+               "%s: the workspace is too small or not 8-byte aligned", who);
   const char* names[3] = {"logprob", "ref_logprob", "mask"};
   for (int i = 0; i < 3; ++i)
     if (int rc = check_stride(who, names[i], row_strides[i], i == 1 && !ref_per_token ? 1 : seq)) return rc;
@@ -327,6 +430,11 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
   a.pairs = pairs; a.seq = seq; a.ref_per_token = ref_per_token != 0; a.splits = splits_for(2 * pairs, seq);
   a.kind = kind; a.average = average != 0; a.beta = beta; a.smoothing = smoothing;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (needed == 0) {
+    a.splits = one_block_splits(2 * pairs);
+    preference_one_block_kernel<<<1, kOneBlock, 0, s>>>(a, seq_grad, rewards, loss);
+    return launch_status("preference_one_block_kernel");
+  }
   auto* part = reinterpret_cast<double*>(workspace);
   preference_kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
   if (int rc = launch_status("preference_kernel")) return rc;

@@ -45,7 +45,7 @@ def _norm_kind(norm_type: float) -> int:
 
 def _items(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]]) -> array:
     """The list as ``molt_grad_item`` records."""
-    if len(set(map(torch.Tensor.get_device, grads))) != 1 or grads[0].device.type != "cuda":
+    if grads[0].device.type != "cuda" or len(set(map(torch.Tensor.get_device, grads))) != 1:
         if any(t.device.type != "cuda" for t in grads):
             raise CapabilityError("gradient norms require CUDA tensors")
         raise ValueError("all gradients must be on one device")
@@ -53,8 +53,7 @@ def _items(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, .
         dtypes = [_DTYPES[t.dtype] for t in grads]
     except KeyError:
         raise CapabilityError("gradient norms support bfloat16 and float32 tensors") from None
-    count = len(grads)
-    flat = [0] * (4 * count)
+    flat = [0] * (4 * len(grads))
     flat[0::4] = map(torch.Tensor.data_ptr, grads)
     if outs is not None:
         flat[1::4] = flat[0::4] if outs is grads else map(torch.Tensor.data_ptr, outs)
@@ -63,30 +62,35 @@ def _items(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, .
     return array("q", flat)
 
 
-@torch.no_grad()
-def global_grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
-    """Norm of all elements of ``grads`` (one tensor or a sequence; bf16 and fp32 may be mixed) as an fp32 scalar on the
-    device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  It is right for every
-    finite gradient, however large or small; a NaN gives NaN, and an infinity infinity.  Equal lists give equal bits."""
-    grads = _checked("grads", grads)
-    kind = _norm_kind(norm_type)
-    items = _items(grads, None)
-    device = grads[0].device
+def _launch(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]], kind: int, max_norm: float) -> torch.Tensor:
+    items, device, count = _items(grads, outs), grads[0].device, len(grads)
     lib = _native.library()
-    scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(len(grads)), device)
+    scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(count), device)
     result = torch.empty(2, dtype=torch.float32, device=device)
     with torch.cuda.device(device):
-        _native.check(lib.molt_grad_norm(items.buffer_info()[0], len(grads), kind, 1.0, float("inf"), result.data_ptr(),
-                                         scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
+        if outs is None:
+            _native.check(lib.molt_grad_norm(items.buffer_info()[0], count, kind, 1.0, max_norm, result.data_ptr(),
+                                             scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
+        else:
+            _native.check(lib.molt_clip_grads(items.buffer_info()[0], count, kind, max_norm, result.data_ptr(),
+                                              scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
     return result[0]
 
 
-@torch.no_grad()
+def global_grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
+    """Norm of all elements of ``grads`` (one tensor or a sequence; bf16 and fp32 may be mixed) as an fp32 scalar on the
+    device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  It is right for every
+    finite gradient, however large or small; a NaN gives NaN, and an infinity infinity.  Equal lists give equal bits.
+    Nothing is recorded for autograd."""
+    grads = _checked("grads", grads)
+    return _launch(grads, None, _norm_kind(norm_type), float("inf"))
+
+
 def clip_grad_norm(grads: Grads, max_norm: float, norm_type: float = 2.0, out: Optional[Grads] = None) -> torch.Tensor:
     """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return their :func:`global_grad_norm` before that.
 
     In place, or into ``out`` (tensors like ``grads``; an output may be its own gradient but must not overlap another
-    tensor of the call).  One tensor must not stand in the list twice."""
+    tensor of the call).  One tensor must not stand in the list twice.  Nothing is recorded for autograd."""
     grads = _checked("grads", grads)
     kind = _norm_kind(norm_type)
     if not max_norm >= 0.0:
@@ -98,13 +102,6 @@ def clip_grad_norm(grads: Grads, max_norm: float, norm_type: float = 2.0, out: O
             raise ValueError("out must match grads in number, shape, dtype and device")
         if any(o.stride() != g.stride() for o, g in zip(outs, grads) if not (o.is_contiguous() and g.is_contiguous())):
             raise ValueError("out must lie in memory as grads do")
-    items = _items(grads, outs)
-    device = grads[0].device
-    lib = _native.library()
-    scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(len(grads)), device)
-    result = torch.empty(2, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        _native.check(lib.molt_clip_grads(items.buffer_info()[0], len(grads), kind, float(max_norm), result.data_ptr(),
-                                          scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))
+    norm = _launch(grads, outs, kind, float(max_norm))
     torch.autograd.graph.increment_version(outs)
-    return result[0]
+    return norm

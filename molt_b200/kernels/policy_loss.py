@@ -24,7 +24,7 @@ class PolicyLoss(NamedTuple):
 
 
 class PreferenceLoss(NamedTuple):
-    """``loss`` is a scalar that carries the gradient, the rewards are ``[pairs]``."""
+    """``loss`` is a scalar that carries the gradient, the rewards are ``[pairs]`` and carry none."""
 
     loss: torch.Tensor
     chosen_rewards: torch.Tensor
@@ -53,7 +53,7 @@ def _check_mask(mask: Optional[torch.Tensor], logprobs: torch.Tensor) -> None:
 
 def _rows(tensor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """The tensor, or a copy where its rows overlap or its tokens are not neighbours (rows may be one and the same)."""
-    if tensor is None or tensor.dim() == 1:
+    if tensor is None or tensor.dim() == 1 or tensor.is_contiguous():
         return tensor
     rows, width = tensor.shape
     neighbours = width <= 1 or tensor.stride(1) == 1
@@ -67,47 +67,52 @@ def _row_stride(tensor: Optional[torch.Tensor]) -> int:
     return tensor.stride(0)
 
 
+def _policy_forward(call, trained: bool):
+    """Loss, ``[k, cut]`` and, for the backward pass, the gradients per token with the weights per sequence behind them."""
+    lp, old, ref, advantages, mask, clip_low, clip_high, kl_coef, reduction = call
+    lp, old, ref, mask, advantages = _rows(lp), _rows(old), _rows(ref), _rows(mask), _rows(advantages)
+    batch, seq = lp.shape
+    device = lp.device
+    loss, stats = lp.new_empty(()), lp.new_empty(2)
+    kept, unit, weight = None, None, None
+    if trained:
+        kept = lp.new_empty(batch * seq + batch)
+        unit = kept.data_ptr()
+        weight = unit + 4 * batch * seq
+    lib = _native.library()
+    nbytes = lib.molt_policy_loss_workspace_bytes(batch, seq)
+    scratch = _native.workspace(nbytes, device) if nbytes else None
+    strides = (ctypes.c_int64 * 5)(*map(_row_stride, (lp, old, ref, advantages, mask)))
+    with torch.cuda.device(device):
+        _native.check(lib.molt_policy_loss_fwd(
+            lp.data_ptr(), old.data_ptr(), _native.ptr(ref), advantages.data_ptr(), int(advantages.dim() == 2),
+            _native.ptr(mask), strides, batch, seq, clip_low, clip_high, kl_coef, reduction, unit, weight, loss.data_ptr(),
+            stats.data_ptr(), _native.ptr(scratch), nbytes, _native.stream_handle(device)))
+    return loss, stats, kept
+
+
 class _PolicyLossFunction(torch.autograd.Function):
-    """Keeps one fp32 value per token and one per sequence for the backward pass."""
+    """Keeps one fp32 value per token and one per sequence for the backward pass; ``told`` receives the statistics."""
 
     @staticmethod
-    def forward(ctx: Any, logprobs, old, ref, advantages, mask, clip_low, clip_high, kl_coef, reduction):
-        batch, seq = logprobs.shape
-        lp, old, ref, mask = _rows(logprobs), _rows(old), _rows(ref), _rows(mask)
-        advantages = _rows(advantages)
-        device = lp.device
-        trained = ctx.needs_input_grad[0]
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        stats = torch.empty(2, dtype=torch.float32, device=device)
-        unit = torch.empty((batch, seq), dtype=torch.float32, device=device) if trained else None
-        weight = torch.empty(batch, dtype=torch.float32, device=device) if trained else None
-        lib = _native.library()
-        scratch = _native.workspace(lib.molt_policy_loss_workspace_bytes(batch, seq), device)
-        strides = (ctypes.c_int64 * 5)(*map(_row_stride, (lp, old, ref, advantages, mask)))
-        with torch.cuda.device(device):
-            _native.check(lib.molt_policy_loss_fwd(
-                lp.data_ptr(), old.data_ptr(), _native.ptr(ref), advantages.data_ptr(), int(advantages.dim() == 2),
-                _native.ptr(mask), strides, batch, seq, clip_low, clip_high, kl_coef, reduction, _native.ptr(unit),
-                _native.ptr(weight), loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                _native.stream_handle(device)))
-        if trained:
-            ctx.save_for_backward(unit, weight)
-        kl, cut = stats[0], stats[1]
-        ctx.mark_non_differentiable(kl, cut)
-        ctx.set_materialize_grads(False)
-        return loss, kl, cut
+    def forward(ctx: Any, logprobs: torch.Tensor, call, told: list) -> torch.Tensor:
+        loss, stats, kept = _policy_forward((logprobs, *call), True)
+        told.append(stats)
+        ctx.save_for_backward(kept)
+        ctx.shape = logprobs.shape
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx: Any, grad_loss, grad_kl, grad_cut):
-        unit, weight = ctx.saved_tensors
-        grad = torch.empty_like(unit)
-        grad_loss = grad_loss.float().contiguous()
-        with torch.cuda.device(unit.device):
-            _native.check(_native.library().molt_policy_loss_bwd(
-                unit.data_ptr(), weight.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(), unit.shape[0], unit.shape[1],
-                _native.stream_handle(unit.device)))
-        return grad, None, None, None, None, None, None, None, None
+    def backward(ctx: Any, grad_loss: torch.Tensor):
+        (kept,) = ctx.saved_tensors
+        batch, seq = ctx.shape
+        grad = kept.new_empty((batch, seq))
+        unit = kept.data_ptr()
+        with torch.cuda.device(kept.device):
+            _native.check(_native.library().molt_policy_loss_bwd(unit, unit + 4 * batch * seq, grad_loss.data_ptr(), grad.data_ptr(),
+                                                                 batch, seq, _native.stream_handle(kept.device)))
+        return grad, None, None
 
 
 def clipped_policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
@@ -131,53 +136,60 @@ def clipped_policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
     _check_mask(mask, logprobs)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
-    return PolicyLoss(*_PolicyLossFunction.apply(logprobs, old_logprobs.detach(),
-                                                 None if ref_logprobs is None else ref_logprobs.detach(), advantages.detach(),
-                                                 mask, float(clip_low), float(clip_high), float(kl_coef),
-                                                 _REDUCTIONS[reduction]))
+    call = (old_logprobs, ref_logprobs, advantages, mask, float(clip_low), float(clip_high), float(kl_coef),
+            _REDUCTIONS[reduction])
+    if logprobs.requires_grad and torch.is_grad_enabled():
+        told: list = []
+        loss = _PolicyLossFunction.apply(logprobs, call, told)
+        stats = told[0]
+    else:
+        loss, stats, _ = _policy_forward((logprobs, *call), False)
+    return PolicyLoss(loss, *stats.unbind())
+
+
+def _preference_forward(call, trained: bool):
+    """Loss, rewards and, for the backward pass, the mask and the gradient of every sequence's tokens."""
+    lp, ref, mask, beta, smoothing, kind, average = call
+    lp, ref, mask = _rows(lp), _rows(ref), _rows(mask)
+    sequences, seq = lp.shape
+    pairs = sequences // 2
+    device = lp.device
+    loss, rewards = lp.new_empty(()), lp.new_empty((2, pairs))
+    seq_grad = lp.new_empty(sequences) if trained else None
+    lib = _native.library()
+    nbytes = lib.molt_preference_loss_workspace_bytes(pairs, seq)
+    scratch = _native.workspace(nbytes, device) if nbytes else None
+    strides = (ctypes.c_int64 * 3)(*map(_row_stride, (lp, ref, mask)))
+    with torch.cuda.device(device):
+        _native.check(lib.molt_preference_loss_fwd(
+            lp.data_ptr(), _native.ptr(ref), int(ref is not None and ref.dim() == 2), _native.ptr(mask), strides, pairs, seq,
+            beta, smoothing, kind, average, _native.ptr(seq_grad), rewards.data_ptr(), loss.data_ptr(), _native.ptr(scratch), nbytes,
+            _native.stream_handle(device)))
+    return loss, rewards, mask, seq_grad
 
 
 class _PreferenceLossFunction(torch.autograd.Function):
-    """Keeps the mask and one fp32 value per sequence for the backward pass."""
+    """Keeps the mask and one fp32 value per sequence for the backward pass; ``told`` receives the rewards."""
 
     @staticmethod
-    def forward(ctx: Any, logprobs, ref, mask, beta, smoothing, kind, average):
-        sequences, seq = logprobs.shape
-        pairs = sequences // 2
-        lp, mask = _rows(logprobs), _rows(mask)
-        ref = _rows(ref)
-        device = lp.device
-        trained = ctx.needs_input_grad[0]
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        rewards = torch.empty((2, pairs), dtype=torch.float32, device=device)
-        seq_grad = torch.empty(sequences, dtype=torch.float32, device=device) if trained else None
-        lib = _native.library()
-        scratch = _native.workspace(lib.molt_preference_loss_workspace_bytes(pairs, seq), device)
-        strides = (ctypes.c_int64 * 3)(*map(_row_stride, (lp, ref, mask)))
-        with torch.cuda.device(device):
-            _native.check(lib.molt_preference_loss_fwd(
-                lp.data_ptr(), _native.ptr(ref), int(ref is not None and ref.dim() == 2), _native.ptr(mask), strides, pairs, seq,
-                beta, smoothing, kind, average, _native.ptr(seq_grad), rewards.data_ptr(), loss.data_ptr(), scratch.data_ptr(),
-                scratch.numel(), _native.stream_handle(device)))
-        if trained:
-            ctx.save_for_backward(mask, seq_grad)
-            ctx.seq = seq
-        chosen, rejected = rewards[0], rewards[1]
-        ctx.mark_non_differentiable(chosen, rejected)
-        ctx.set_materialize_grads(False)
-        return loss, chosen, rejected
+    def forward(ctx: Any, logprobs: torch.Tensor, call, told: list) -> torch.Tensor:
+        loss, rewards, mask, seq_grad = _preference_forward((logprobs, *call), True)
+        told.append(rewards)
+        ctx.save_for_backward(mask, seq_grad)
+        ctx.shape = logprobs.shape
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx: Any, grad_loss, grad_chosen, grad_rejected):
+    def backward(ctx: Any, grad_loss: torch.Tensor):
         mask, seq_grad = ctx.saved_tensors
-        grad = torch.empty((seq_grad.shape[0], ctx.seq), dtype=torch.float32, device=seq_grad.device)
-        grad_loss = grad_loss.float().contiguous()
+        sequences, seq = ctx.shape
+        grad = seq_grad.new_empty((sequences, seq))
         with torch.cuda.device(grad.device):
             _native.check(_native.library().molt_preference_loss_bwd(
-                _native.ptr(mask), _row_stride(mask), seq_grad.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(),
-                grad.shape[0] // 2, ctx.seq, _native.stream_handle(grad.device)))
-        return grad, None, None, None, None, None, None
+                _native.ptr(mask), _row_stride(mask), seq_grad.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(), sequences // 2, seq,
+                _native.stream_handle(grad.device)))
+        return grad, None, None
 
 
 def preference_loss(logprobs: torch.Tensor, ref_logprobs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
@@ -201,5 +213,11 @@ def preference_loss(logprobs: torch.Tensor, ref_logprobs: Optional[torch.Tensor]
     _check_mask(mask, logprobs)
     if kind not in _KINDS:
         raise ValueError(f"kind must be one of {sorted(_KINDS)}")
-    return PreferenceLoss(*_PreferenceLossFunction.apply(logprobs, None if ref_logprobs is None else ref_logprobs.detach(), mask,
-                                                         float(beta), float(label_smoothing), _KINDS[kind], int(bool(average))))
+    call = (ref_logprobs, mask, float(beta), float(label_smoothing), _KINDS[kind], int(bool(average)))
+    if logprobs.requires_grad and torch.is_grad_enabled():
+        told: list = []
+        loss = _PreferenceLossFunction.apply(logprobs, call, told)
+        rewards = told[0]
+    else:
+        loss, rewards, _, _ = _preference_forward((logprobs, *call), False)
+    return PreferenceLoss(loss, *rewards.unbind())

@@ -69,13 +69,13 @@ def test_token_logprob_of_no_rows_is_no_launch(native_library):
     ({"high": float("nan")}, _native.E_VALUE, "clip_high"), ({"kl": float("nan")}, _native.E_VALUE, "kl_coef"),
     ({"reduction": 2}, _native.E_VALUE, "reduction"), ({"lp": None}, _native.E_VALUE, "NULL"), ({"old": None}, _native.E_VALUE, "NULL"),
     ({"adv": None}, _native.E_VALUE, "NULL"), ({"loss": None}, _native.E_VALUE, "NULL"), ({"stats": None}, _native.E_VALUE, "NULL"),
-    ({"unit": None}, _native.E_VALUE, "NULL"), ({"weight": None}, _native.E_VALUE, "NULL"), ({"ws": None}, _native.E_VALUE, "NULL"),
+    ({"unit": None}, _native.E_VALUE, "NULL"), ({"weight": None}, _native.E_VALUE, "NULL"), ({"ws": None}, _native.E_VALUE, "workspace"),
     ({"ws": E + 4}, _native.E_VALUE, "workspace"), ({"ws_bytes": 8}, _native.E_VALUE, "workspace"),
     ({"strides": (15, 16, 16, 16, 16)}, _native.E_VALUE, "logprob"), ({"strides": (16, 16, 16, 16, 15)}, _native.E_VALUE, "mask"),
     ({"strides": (16, 16, 16, 15, 16)}, _native.E_VALUE, "advantage"), ({"strides": (16, 16, 16, -1, 16), "per_token": 0},
                                                                         _native.E_VALUE, "advantage")])
 def test_policy_loss_refusals(native_library, change, expected, word):
-    c = dict(lp=A, old=B, ref=C, adv=D, per_token=1, mask=None, strides=(16,) * 5, batch=4, seq=16, low=0.2, high=0.2, kl=0.1,
+    c = dict(lp=A, old=B, ref=C, adv=D, per_token=1, mask=None, strides=(16,) * 5, batch=600, seq=16, low=0.2, high=0.2, kl=0.1,
              reduction=0, unit=A + 0x1000, weight=A + 0x2000, loss=A + 0x3000, stats=A + 0x4000, ws=E, ws_bytes=1 << 20)
     c.update(change)
     rc = native_library.molt_policy_loss_fwd(c["lp"], c["old"], c["ref"], c["adv"], c["per_token"], c["mask"],
@@ -99,12 +99,12 @@ def test_policy_backward_refusals(native_library):
     ({"beta": float("inf")}, _native.E_VALUE, "beta"), ({"smoothing": -0.1}, _native.E_VALUE, "smoothing"),
     ({"smoothing": 1.1}, _native.E_VALUE, "smoothing"), ({"smoothing": 0.1, "kind": 1}, _native.E_VALUE, "smoothing"),
     ({"kind": 3}, _native.E_VALUE, "kind"), ({"lp": None}, _native.E_VALUE, "NULL"), ({"rewards": None}, _native.E_VALUE, "NULL"),
-    ({"loss": None}, _native.E_VALUE, "NULL"), ({"ws": None}, _native.E_VALUE, "NULL"), ({"ws": E + 4}, _native.E_VALUE, "workspace"),
+    ({"loss": None}, _native.E_VALUE, "NULL"), ({"ws": None}, _native.E_VALUE, "workspace"), ({"ws": E + 4}, _native.E_VALUE, "workspace"),
     ({"ws_bytes": 8}, _native.E_VALUE, "workspace"), ({"strides": (7, 8, 8)}, _native.E_VALUE, "logprob"),
     ({"strides": (8, 7, 8)}, _native.E_VALUE, "ref_logprob"), ({"strides": (8, -1, 8), "per_token": 0}, _native.E_VALUE, "ref_logprob"),
     ({"strides": (8, 8, 7)}, _native.E_VALUE, "mask")])
 def test_preference_loss_refusals(native_library, change, expected, word):
-    c = dict(lp=A, ref=B, per_token=1, mask=C, strides=(8, 8, 8), pairs=2, seq=8, beta=0.1, smoothing=0.0, kind=0, average=0,
+    c = dict(lp=A, ref=B, per_token=1, mask=C, strides=(8, 8, 8), pairs=200, seq=8, beta=0.1, smoothing=0.0, kind=0, average=0,
              grad=D, rewards=D + 0x1000, loss=D + 0x2000, ws=E, ws_bytes=1 << 20)
     c.update(change)
     rc = native_library.molt_preference_loss_fwd(c["lp"], c["ref"], c["per_token"], c["mask"], _strides(*c["strides"]), c["pairs"],
