@@ -55,7 +55,7 @@ struct PolicyArgs {
   long long batch, seq;
   int per_token, splits;
   double log_high, log_low;   // ln(1 + clip_high), ln(1 - clip_low): the borders of ln r
-  float high, low, kl_coef;   // 1 + clip_high, 1 - clip_low
+  float log_high_f, log_low_f, high, low, kl_coef;   // the borders rounded to fp32; 1 + clip_high, 1 - clip_low
 };
 
 // exp(d) - 1 - d without the cancellation: the Taylor series d^2/2 (1 + d/3 (1 + d/4 (...))) where |d| is small (its
@@ -89,30 +89,42 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
         kept[j] = a.mask == nullptr || a.mask[b * a.mask_stride + t] != 0;
       }
     }
+    float loss = 0.f, ks = 0.f;
+    int cuts = 0, keeps = 0;
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       float g = 0.f;
       if (kept[j]) {
-        const double d = (double)lp[j] - (double)old[j];
-        const bool cut = (adv[j] > 0.f && d > a.log_high) || (adv[j] < 0.f && d < a.log_low);
+        // fp32 rounds monotonously, so the rounded difference decides the border unless it lies on it
+        const float d = lp[j] - old[j];
+        bool cut = (adv[j] > 0.f && d > a.log_high_f) || (adv[j] < 0.f && d < a.log_low_f);
+        if (d == a.log_high_f || d == a.log_low_f) {
+          const double exact = (double)lp[j] - (double)old[j];
+          cut = (adv[j] > 0.f && exact > a.log_high) || (adv[j] < 0.f && exact < a.log_low);
+        }
         float l = 0.f;
         if (adv[j] != 0.f) {   // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
-          const float r = expf((float)d);
+          const float r = expf(d);
           l = -(cut ? (adv[j] > 0.f ? a.high : a.low) : r) * adv[j];
           g = cut ? 0.f : -r * adv[j];
         }
         if (a.ref != nullptr) {
           const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
           l += a.kl_coef * k;
-          g -= a.kl_coef * expm1f(e);
-          sum[1] += k;
+          g -= a.kl_coef * (k + e);   // exp(e) - 1
+          ks += k;
         }
-        sum[0] += l;
-        sum[2] += cut ? 1. : 0.;
-        sum[3] += 1.;
+        loss += l;
+        cuts += cut;
+        ++keeps;
       }
       if (unit_grad != nullptr && t0 + j * step < end) unit_grad[b * a.seq + t0 + j * step] = g;
     }
+    // four tokens in fp32, then in 64 bits: three roundings more on values that carry a few already
+    sum[0] += loss;
+    sum[1] += ks;
+    sum[2] += cuts;
+    sum[3] += keeps;
   }
 }
 
@@ -121,20 +133,30 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
                                               float* __restrict__ row_weight, float* __restrict__ loss,
                                               float* __restrict__ stats) {
   __shared__ double total;
+  const auto row_sum = [&](long long b, double (&row)[4]) {
+    for (int i = 0; i < 4; ++i) row[i] = 0.;
+    for (int s = 0; s < splits; ++s)
+      for (int i = 0; i < 4; ++i) row[i] += part[(b * splits + s) * 4 + i];
+  };
+  // a thread's first row is read once; rows beyond the block's size a second time
+  double first[4] = {0., 0., 0., 0.}, row[4];
   double count[1] = {0.};
   for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
-    double kept = 0.;
-    for (int s = 0; s < splits; ++s) kept += part[(b * splits + s) * 4 + 3];
-    count[0] += reduction == MOLT_REDUCE_TOKEN ? kept : (kept > 0. ? 1. : 0.);
+    row_sum(b, row);
+    if (b < blockDim.x)
+      for (int i = 0; i < 4; ++i) first[i] = row[i];
+    count[0] += reduction == MOLT_REDUCE_TOKEN ? row[3] : (row[3] > 0. ? 1. : 0.);
   }
   block_sum(count);
   if (threadIdx.x == 0) total = count[0];
   __syncthreads();
   double sum[3] = {0., 0., 0.};
   for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
-    double row[4] = {0., 0., 0., 0.};
-    for (int s = 0; s < splits; ++s)
-      for (int i = 0; i < 4; ++i) row[i] += part[(b * splits + s) * 4 + i];
+    if (b < blockDim.x) {
+      for (int i = 0; i < 4; ++i) row[i] = first[i];
+    } else {
+      row_sum(b, row);
+    }
     double w = 0.;
     if (row[3] > 0.) {
       w = reduction == MOLT_REDUCE_TOKEN ? 1. / total : 1. / (total * row[3]);
@@ -186,18 +208,21 @@ __global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs 
   policy_finish(part, a.batch, a.splits, reduction, row_weight, loss, stats);
 }
 
+// Backward passes: a thread takes kUnroll tokens of one row, so that a block is one round of loads and stores.
+constexpr int kBackTokens = kThreads * kUnroll;
+
 __global__ void __launch_bounds__(kThreads) policy_backward_kernel(const float* __restrict__ unit_grad,
                                                                    const float* __restrict__ row_weight,
                                                                    const float* __restrict__ grad_loss,
-                                                                   float* __restrict__ grad_logprob, long long seq, int splits) {
-  const long long b = blockIdx.x;
-  const long long begin = seq * blockIdx.y / splits, end = seq * (blockIdx.y + 1) / splits;
+                                                                   float* __restrict__ grad_logprob, long long seq) {
+  const long long b = blockIdx.x, first = b * seq, t0 = (long long)blockIdx.y * kBackTokens + threadIdx.x;
+  float u[kUnroll];
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) u[j] = t0 + j * kThreads < seq ? unit_grad[first + t0 + j * kThreads] : 0.f;
   const float w = row_weight[b] * grad_loss[0];
-#pragma unroll 4
-  for (long long t = begin + threadIdx.x; t < end; t += kThreads) {
-    const float u = unit_grad[b * seq + t];
-    grad_logprob[b * seq + t] = u == 0.f ? 0.f : u * w;
-  }
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j)
+    if (t0 + j * kThreads < seq) grad_logprob[first + t0 + j * kThreads] = u[j] == 0.f ? 0.f : u[j] * w;
 }
 
 // ---- preference pairs ----------------------------------------------------------------------------------------------
@@ -212,6 +237,7 @@ struct PreferenceArgs {
 
 __device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long long i, long long begin, long long end, int step,
                                                   double (&sum)[2]) {
+  int keeps = 0;
   for (long long t0 = begin; t0 < end; t0 += kUnroll * step) {
     float lp[kUnroll], ref[kUnroll];
     bool kept[kUnroll];
@@ -226,12 +252,14 @@ __device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long 
       }
     }
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j)
-      if (kept[j]) {
-        sum[0] += (double)lp[j] - (double)ref[j];
-        sum[1] += 1.;
-      }
+    for (int j = 0; j < kUnroll; j += 2) {
+      // a pair of fp32 differences is added before it goes on in 64 bits: two roundings of the terms' magnitudes
+      const float d0 = kept[j] ? lp[j] - ref[j] : 0.f, d1 = kept[j + 1] ? lp[j + 1] - ref[j + 1] : 0.f;
+      sum[0] += d0 + d1;
+      keeps += (int)kept[j] + (int)kept[j + 1];
+    }
   }
+  sum[1] += keeps;
 }
 
 __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const double* part, float* __restrict__ seq_grad,
@@ -317,18 +345,21 @@ __global__ void __launch_bounds__(kOneBlock) preference_one_block_kernel(Prefere
 __global__ void __launch_bounds__(kThreads) preference_backward_kernel(const uint8_t* __restrict__ mask, long long mask_stride,
                                                                        const float* __restrict__ seq_grad,
                                                                        const float* __restrict__ grad_loss,
-                                                                       float* __restrict__ grad_logprob, long long seq, int splits) {
-  const long long i = blockIdx.x;
-  const long long begin = seq * blockIdx.y / splits, end = seq * (blockIdx.y + 1) / splits;
+                                                                       float* __restrict__ grad_logprob, long long seq) {
+  const long long i = blockIdx.x, t0 = (long long)blockIdx.y * kBackTokens + threadIdx.x;
+  bool kept[kUnroll];
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j)
+    kept[j] = t0 + j * kThreads < seq && (mask == nullptr || mask[i * mask_stride + t0 + j * kThreads] != 0);
   const float g = seq_grad[i] * grad_loss[0];
-#pragma unroll 4
-  for (long long t = begin + threadIdx.x; t < end; t += kThreads)
-    grad_logprob[i * seq + t] = mask == nullptr || mask[i * mask_stride + t] != 0 ? g : 0.f;
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j)
+    if (t0 + j * kThreads < seq) grad_logprob[i * seq + t0 + j * kThreads] = kept[j] ? g : 0.f;
 }
 
 int check_sizes(const char* who, int64_t rows, int64_t seq) {
   MOLT_REQUIRE(rows >= 0 && seq >= 0, MOLT_E_VALUE, "%s: negative size", who);
-  MOLT_REQUIRE(rows < (1LL << 31) && seq <= (1LL << 31), MOLT_E_CAPABILITY, "%s: 2^31 sequences or more than 2^31 tokens in one", who);
+  MOLT_REQUIRE(rows < (1LL << 31) && seq <= (1LL << 25), MOLT_E_CAPABILITY, "%s: 2^31 sequences or more than 2^25 tokens in one", who);
   return MOLT_OK;
 }
 
@@ -375,6 +406,7 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
   a.mask_stride = row_strides[4];
   a.batch = batch; a.seq = seq; a.per_token = advantage_per_token != 0; a.splits = splits_for(batch, seq);
   a.log_high = log1p(clip_high); a.log_low = log1p(-clip_low);
+  a.log_high_f = (float)a.log_high; a.log_low_f = (float)a.log_low;
   a.high = (float)(1. + clip_high); a.low = (float)(1. - clip_low); a.kl_coef = (float)kl_coef;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (needed == 0) {
@@ -395,9 +427,9 @@ extern "C" int molt_policy_loss_bwd(const float* unit_grad, const float* row_wei
   if (int rc = check_sizes(who, batch, seq)) return rc;
   if (batch == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(unit_grad && row_weight && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
-  const int splits = splits_for(batch, seq);
-  policy_backward_kernel<<<dim3((unsigned)batch, splits), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      unit_grad, row_weight, grad_loss, grad_logprob, seq, splits);
+  const dim3 grid((unsigned)batch, (unsigned)((seq + kBackTokens - 1) / kBackTokens));
+  policy_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(unit_grad, row_weight, grad_loss, grad_logprob,
+                                                                                       seq);
   return launch_status("policy_backward_kernel");
 }
 
@@ -450,8 +482,8 @@ extern "C" int molt_preference_loss_bwd(const uint8_t* mask, int64_t mask_stride
   if (pairs == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(seq_grad && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   if (int rc = check_stride(who, "mask", mask_stride, seq)) return rc;
-  const int splits = splits_for(2 * pairs, seq);
-  preference_backward_kernel<<<dim3((unsigned)(2 * pairs), splits), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      mask, mask_stride, seq_grad, grad_loss, grad_logprob, seq, splits);
+  const dim3 grid((unsigned)(2 * pairs), (unsigned)((seq + kBackTokens - 1) / kBackTokens));
+  preference_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(mask, mask_stride, seq_grad, grad_loss,
+                                                                                           grad_logprob, seq);
   return launch_status("preference_backward_kernel");
 }

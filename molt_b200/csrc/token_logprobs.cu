@@ -59,6 +59,7 @@ struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int kElements = 4;
+  static constexpr unsigned kMinusInf = 0xff800000u;
   static __device__ __forceinline__ float largest(const uint4& q, float m) {
     return fmaxf(fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w))), m);
   }
@@ -77,6 +78,7 @@ struct Vec<float> {
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int kElements = 8;
+  static constexpr unsigned kMinusInf = 0xff80ff80u;
   static __device__ __forceinline__ unsigned max2(unsigned a, unsigned b) {   // drops a NaN, which the sum then carries
     unsigned r;
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -236,25 +238,22 @@ __device__ __forceinline__ bool cut_alike(const T* a, const T* b) {
   return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-// One row per cluster of blocks (of one block, when there are enough rows).  First pass: the running pair over the
-// block's vectors, NB of them at a time.  GRAD: second pass, from the last vector to the first, over the same vectors, which
-// the L2 still holds.
-template <typename T, bool GRAD, int THREADS, int NB, int BLOCKS>
+// Log-probabilities alone: a row per block, or per cluster of blocks when there are too few rows to fill the device.  HBM-bound:
+// 2048 rows of 151936 bf16 logits take 97 us (6.4 TB/s).  512 threads with 4 vectors each in flight, 4 blocks per SM;
+// 256 threads were 2-4 % slower, 8 vectors 10 %.
+template <typename T, int THREADS, int NB, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
-    row_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids, const float* __restrict__ weight,
-               float inv_t, float* __restrict__ logprob, float2* __restrict__ stats, T* grad, long long grad_stride, int vocab) {
-  constexpr int E = Vec<T>::kElements;
+    row_kernel(const T* __restrict__ logits, long long row_stride, const long long* __restrict__ ids, float inv_t,
+               float* __restrict__ logprob, float2* __restrict__ stats, int vocab) {
   const unsigned size = cluster_size(), rank = cluster_rank();
   const long long row = blockIdx.x / size, t = ids[row];
   const T* x = logits + row * row_stride;
-  T* g = GRAD ? grad + row * grad_stride : nullptr;
   const int first = rank * THREADS + threadIdx.x, step = size * THREADS;
   if (t < 0 || t >= vocab) {
     if (first == 0) {
       logprob[row] = 0.f;
-      if (!GRAD && stats != nullptr) stats[row] = make_float2(0.f, 0.f);
+      if (stats != nullptr) stats[row] = make_float2(0.f, 0.f);
     }
-    if (GRAD) clear(g, 0, vocab, first, step);
     return;
   }
   if (size > 1) cluster_arrive();
@@ -268,47 +267,131 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   for (; v + (NB - 1) * step < cut.vectors; v += NB * step) {
     uint4 q[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) q[j] = GRAD ? p[v + j * step] : __ldcs(p + v + j * step);
+    for (int j = 0; j < NB; ++j) q[j] = __ldcs(p + v + j * step);
     run.template take<T, NB>(q);
   }
-  const int whole = v;
   for (; v < cut.vectors; v += step) {
-    const uint4 q[1] = {GRAD ? p[v] : __ldcs(p + v)};
+    const uint4 q[1] = {__ldcs(p + v)};
     run.template take<T, 1>(q);
   }
-  float loose_x = 0.f;
-  if (loose >= 0) {
-    loose_x = load1(x + loose);
-    run.take_one(loose_x);
+  if (loose >= 0) run.take_one(load1(x + loose));
+  const float2 sums = halves(run.s);
+  float m = run.m, s = sums.x + sums.y;
+  row_join<THREADS>(m, s, run.c, rank, size);
+  if (first == 0) {
+    const float log2_s = log2f(s);
+    logprob[row] = (xt - m) * inv_t - log2_s * kLn2;
+    if (stats != nullptr) stats[row] = make_float2(m, log2_s);
   }
+}
+
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Log-probabilities and gradient in one kernel.  Bound by HBM in principle (each logit read and each gradient written
+// once) and by latency in practice, since no gradient can be formed before the whole row has been seen.  A row does not fit
+// one SM (151936 bf16 logits are 304 KB), so a cluster of blocks shares it, and the second pass reads it again from the L2:
+// 5 blocks of 256 threads per SM, at most 20 vectors per thread, keep 60 MB of rows in flight.  What keeps the loads going is
+// a ring of RING batches of B vectors per thread in shared memory, filled by asynchronous copies that each thread makes for
+// itself (no barrier): the first pass runs it upwards, the second one downwards, beginning with the batches that it still
+// holds.  2048 rows of 151936 bf16: 212 us (5.9 TB/s of 6.55).  Other forms, same rows: loads through registers 232, rows
+// held in the registers of a cluster 291-388, in its shared memory 253-390 (the join of the row then leaves the memory
+// idle), persistent blocks that fetch their next row early 231-296, two kernels (forward, then backward_kernel) 280.
+constexpr int kRing = 5, kRingBatch = 2;
+
+template <typename T, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
+    row_grad_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids, const float* __restrict__ weight,
+                    float inv_t, float* __restrict__ logprob, T* grad, long long grad_stride, int vocab) {
+  constexpr int E = Vec<T>::kElements, B = kRingBatch;
+  extern __shared__ uint4 ring[];   // [kRing * B][THREADS]
+  const unsigned size = cluster_size(), rank = cluster_rank();
+  const long long row = blockIdx.x / size, t = ids[row];
+  const T* x = logits + row * row_stride;
+  T* g = grad + row * grad_stride;
+  const int first = rank * THREADS + threadIdx.x, step = size * THREADS;
+  if (t < 0 || t >= vocab) {
+    if (first == 0) logprob[row] = 0.f;
+    clear(g, 0, vocab, first, step);
+    return;
+  }
+  if (size > 1) cluster_arrive();
+  const Cut<T> cut(x, vocab);
+  const uint4* p = reinterpret_cast<const uint4*>(x + cut.head);
+  uint4* mine = ring + threadIdx.x;
+  const int batches = ((cut.vectors + step - 1) / step + B - 1) / B;   // the same for every thread of the row
+  const auto fetch = [&](int k, int slot) {
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int v = first + (k * B + j) * step;
+      if (v < cut.vectors) copy_async(mine + (slot * B + j) * THREADS, p + v);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kRing; ++k) {
+    if (k < batches) fetch(k, k);
+    copy_commit();
+  }
+  const int loose = first < 16 ? cut.loose(first, vocab) : -1;
+  const float loose_x = loose >= 0 ? load1(x + loose) : 0.f;
+  const float w = (weight != nullptr ? weight[row] : 1.f) * inv_t;
+  Running run;
+  run.c = inv_t * kLog2e;
+  int slot = 0;
+  for (int k = 0; k < batches; ++k) {
+    copy_wait<kRing - 1>();
+    uint4 q[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      q[j] = first + (k * B + j) * step < cut.vectors
+                 ? mine[(slot * B + j) * THREADS]
+                 : make_uint4(Vec<T>::kMinusInf, Vec<T>::kMinusInf, Vec<T>::kMinusInf, Vec<T>::kMinusInf);
+    run.template take<T, B>(q);
+    if (k + kRing < batches) fetch(k + kRing, slot);   // into the slot that has just been read
+    copy_commit();
+    slot = slot + 1 == kRing ? 0 : slot + 1;
+  }
+  if (loose >= 0) run.take_one(loose_x);
   const float2 sums = halves(run.s);
   float m = run.m, s = sums.x + sums.y;
   row_join<THREADS>(m, s, run.c, rank, size);
   const float log2_s = log2f(s);
-  const float l = (xt - m) * inv_t - log2_s * kLn2;
-  if (first == 0) {
+  const pair_t minus = pair(-m, -m), cc = pair(run.c, run.c), less = pair(-log2_s, -log2_s), scale = pair(-w, -w);
+  const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
+  // the target's own column, by the thread that holds it: 1 - p without the cancellation
+  const auto target = [&](float xt) {
+    const float l = (xt - m) * inv_t - log2_s * kLn2;
     logprob[row] = l;
-    if (!GRAD && stats != nullptr) stats[row] = make_float2(m, log2_s);
-  }
-  if (GRAD) {
-    const float w = (weight != nullptr ? weight[row] : 1.f) * inv_t;
-    const pair_t minus = pair(-m, -m), cc = pair(run.c, run.c), less = pair(-log2_s, -log2_s), scale = pair(-w, -w);
-    const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
-    const bool alike = cut_alike(x, g);
-    T* to = g + cut.head;
-    for (v -= step; v >= whole; v -= step) put(to + (long long)v * E, Vec<T>::map(__ldcs(p + v), f), alike);
-    for (v = whole - NB * step; v >= 0; v -= NB * step) {
-      uint4 q[NB];
+    store1(g + t, -expm1f(l) * w);
+  };
+  const bool alike = cut_alike(x, g);
+  const int at = (int)t - cut.head;
+  const int holder = at >= 0 && at / E < cut.vectors ? at / E : -1;
+  T* to = g + cut.head;
+  for (int k = batches - 1; k >= 0; --k) {
+    slot = slot == 0 ? kRing - 1 : slot - 1;
+    copy_wait<kRing - 1>();
 #pragma unroll
-      for (int j = 0; j < NB; ++j) q[j] = __ldcs(p + v + j * step);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) put(to + (long long)(v + j * step) * E, Vec<T>::map(q[j], f), alike);
+    for (int j = 0; j < B; ++j) {
+      const int v = first + (k * B + j) * step;
+      if (v < cut.vectors) {
+        const uint4* held = mine + (slot * B + j) * THREADS;
+        put(to + (long long)v * E, Vec<T>::map(*held, f), alike);
+        if (v == holder) target(load1(reinterpret_cast<const T*>(held) + (at - v * E)));
+      }
     }
-    if (loose >= 0) store1(g + loose, exp2_fast((loose_x - m) * run.c - log2_s) * -w);
-    // the target's own column, by the thread that has just written it: 1 - p without the cancellation
-    const int at = (int)t - cut.head, holder = at / E;
-    const bool own = at >= 0 && holder < cut.vectors ? holder % step == first : loose == (int)t;
-    if (own) store1(g + t, -expm1f(l) * w);
+    if (k >= kRing) fetch(k - kRing, slot);
+    copy_commit();
+  }
+  if (loose >= 0) {
+    if (loose == (int)t) target(loose_x);
+    else store1(g + loose, exp2_fast((loose_x - m) * run.c - log2_s) * -w);
   }
 }
 
@@ -399,13 +482,13 @@ int check_grad(const char* who, const void* logits, int dtype, int64_t row_strid
   return fail(MOLT_E_VALUE, "%s: the gradient overlaps the logits without being the same rows", who);
 }
 
-template <typename T, bool GRAD, int THREADS, int NB, int BLOCKS>
-int launch_row_kernel(int cluster, const void* logits, int64_t row_stride, const int64_t* ids, const float* weight,
-                      float temperature, float* logprob, float* stats, void* grad, int64_t grad_stride, int64_t rows,
-                      int64_t vocab, cudaStream_t s) {
+template <typename... Params, typename... Args>
+int launch_clusters(const char* what, void (*kernel)(Params...), int64_t rows, int cluster, int threads, size_t shared, cudaStream_t s,
+                    Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(rows * cluster));
-  config.blockDim = dim3(THREADS);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
   config.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -414,28 +497,45 @@ int launch_row_kernel(int cluster, const void* logits, int64_t row_stride, const
   attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&config, row_kernel<T, GRAD, THREADS, NB, BLOCKS>, reinterpret_cast<const T*>(logits), (long long)row_stride,
-                     reinterpret_cast<const long long*>(ids), weight, 1.f / temperature, logprob, reinterpret_cast<float2*>(stats),
-                     reinterpret_cast<T*>(grad), (long long)grad_stride, (int)vocab);
-  return launch_status("token_logprob row_kernel");
+  cudaLaunchKernelEx(&config, kernel, Params(args)...);
+  return launch_status(what);
+}
+
+// Rows of at most 512 vectors (4096 bf16, 2048 fp32) take small blocks, many to an SM; longer ones large blocks, and a
+// cluster of them (a power of two, at most 8) where one block would not do:
+// * with gradient, until a thread has at most 20 vectors, so that the rows in flight stay in the L2;
+// * in both directions, as long as the rows alone do not fill the device and a thread keeps at least 4 vectors.
+template <typename T>
+int launch_forward(const void* logits, int64_t row_stride, const int64_t* ids, float temperature, float* logprob, float* stats,
+                   int64_t rows, int64_t vocab, cudaStream_t s) {
+  const int64_t vectors = vocab / Vec<T>::kElements;
+  auto* x = reinterpret_cast<const T*>(logits);
+  auto* id = reinterpret_cast<const long long*>(ids);
+  auto* st = reinterpret_cast<float2*>(stats);
+  if (vectors <= 64 * 8)
+    return launch_clusters("token_logprob row_kernel", row_kernel<T, 64, 2, 16>, rows, 1, 64, 0, s, x, row_stride, id, 1.f / temperature,
+                           logprob, st, vocab);
+  int cluster = 1;
+  while (cluster < 8 && rows * cluster < 148 * 2 && vectors >= cluster * 512 * 4) cluster *= 2;
+  return launch_clusters("token_logprob row_kernel", row_kernel<T, 512, 4, sizeof(T) == 2 ? 4 : 3>, rows, cluster, 512, 0, s, x, row_stride,
+                         id, 1.f / temperature, logprob, st, vocab);
 }
 
 template <typename T>
-int launch_rows(const void* logits, int64_t row_stride, const int64_t* ids, const float* weight, float temperature,
-                float* logprob, float* stats, void* grad, int64_t grad_stride, int64_t rows, int64_t vocab, cudaStream_t s) {
+int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, const float* weight, float temperature, float* logprob,
+                void* grad, int64_t grad_stride, int64_t rows, int64_t vocab, cudaStream_t s) {
+  constexpr size_t kSlots = kRing * kRingBatch * sizeof(uint4);
   const int64_t vectors = vocab / Vec<T>::kElements;
-#define MOLT_ROWS(GRAD, THREADS, NB, BLOCKS, CLUSTER)                                                                       \
-  launch_row_kernel<T, GRAD, THREADS, NB, BLOCKS>(CLUSTER, logits, row_stride, ids, weight, temperature, logprob, stats, grad, \
-                                                  grad_stride, rows, vocab, s)
-  if (vectors <= 64 * 8) return grad != nullptr ? MOLT_ROWS(true, 64, 2, 16, 1) : MOLT_ROWS(false, 64, 2, 16, 1);
+  auto* x = reinterpret_cast<const T*>(logits);
+  auto* id = reinterpret_cast<const long long*>(ids);
+  auto* g = reinterpret_cast<T*>(grad);
+  if (vectors <= 64 * 8)
+    return launch_clusters("token_logprob row_grad_kernel", row_grad_kernel<T, 64, 16>, rows, 1, 64, 64 * kSlots, s, x, row_stride, id,
+                           weight, 1.f / temperature, logprob, g, grad_stride, vocab);
   int cluster = 1;
-  if (grad != nullptr) {
-    while (cluster < 8 && (vectors > cluster * 256 * 20 || (rows * cluster < 148 * 4 && vectors >= cluster * 256 * 4))) cluster *= 2;
-    return MOLT_ROWS(true, 256, 4, 5, cluster);
-  }
-  while (cluster < 8 && rows * cluster < 148 * 2 && vectors >= cluster * 512 * 4) cluster *= 2;
-  return MOLT_ROWS(false, 512, 4, (sizeof(T) == 2 ? 4 : 3), cluster);
-#undef MOLT_ROWS
+  while (cluster < 8 && (vectors > cluster * 256 * 20 || (rows * cluster < 148 * 4 && vectors >= cluster * 256 * 4))) cluster *= 2;
+  return launch_clusters("token_logprob row_grad_kernel", row_grad_kernel<T, 256, 5>, rows, cluster, 256, 256 * kSlots, s, x, row_stride, id,
+                         weight, 1.f / temperature, logprob, g, grad_stride, vocab);
 }
 
 }  // namespace
@@ -451,8 +551,8 @@ extern "C" int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row
   MOLT_REQUIRE(logprob != nullptr, MOLT_E_VALUE, "molt_token_logprob_fwd: NULL tensor pointer");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == MOLT_DTYPE_BF16
-             ? launch_rows<__nv_bfloat16>(logits, row_stride, token_ids, nullptr, temperature, logprob, stats, nullptr, 0, rows, vocab, s)
-             : launch_rows<float>(logits, row_stride, token_ids, nullptr, temperature, logprob, stats, nullptr, 0, rows, vocab, s);
+             ? launch_forward<__nv_bfloat16>(logits, row_stride, token_ids, temperature, logprob, stats, rows, vocab, s)
+             : launch_forward<float>(logits, row_stride, token_ids, temperature, logprob, stats, rows, vocab, s);
 }
 
 extern "C" int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids,
@@ -464,10 +564,10 @@ extern "C" int molt_token_logprob_grad(const void* logits, int dtype, int64_t ro
   if (rows == 0) return MOLT_OK;
   MOLT_REQUIRE(logprob != nullptr, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == MOLT_DTYPE_BF16 ? launch_rows<__nv_bfloat16>(logits, row_stride, token_ids, weight, temperature, logprob, nullptr,
-                                                               grad_logits, grad_stride, rows, vocab, s)
-                                  : launch_rows<float>(logits, row_stride, token_ids, weight, temperature, logprob, nullptr,
-                                                       grad_logits, grad_stride, rows, vocab, s);
+  return dtype == MOLT_DTYPE_BF16 ? launch_grad<__nv_bfloat16>(logits, row_stride, token_ids, weight, temperature, logprob, grad_logits,
+                                                               grad_stride, rows, vocab, s)
+                                  : launch_grad<float>(logits, row_stride, token_ids, weight, temperature, logprob, grad_logits,
+                                                       grad_stride, rows, vocab, s);
 }
 
 extern "C" int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids,

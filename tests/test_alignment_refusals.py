@@ -64,6 +64,7 @@ def test_token_logprob_of_no_rows_is_no_launch(native_library):
 @pytest.mark.parametrize("change,expected,word", [
     ({"batch": 0}, _native.E_VALUE, "no sequence"), ({"batch": -1}, _native.E_VALUE, "negative"),
     ({"seq": -1}, _native.E_VALUE, "negative"), ({"batch": 1 << 31}, _native.E_CAPABILITY, "2^31"),
+    ({"seq": (1 << 25) + 1}, _native.E_CAPABILITY, "2^25"),
     ({"low": -0.1}, _native.E_VALUE, "clip_low"), ({"low": 1.1}, _native.E_VALUE, "clip_low"),
     ({"high": -0.1}, _native.E_VALUE, "clip_high"), ({"high": float("inf")}, _native.E_VALUE, "clip_high"),
     ({"high": float("nan")}, _native.E_VALUE, "clip_high"), ({"kl": float("nan")}, _native.E_VALUE, "kl_coef"),
