@@ -322,7 +322,7 @@ int molt_mlp_bwd_t(const molt_lora_proj* gate, const molt_lora_proj* up, const m
  *   logprob[r] = (x[t] - max) / T - ln(sum_v exp((x[v] - max) / T)),   t = token_ids[r], T = temperature.
  * A token id outside [0, vocab) (an ignore index such as -100) gives 0 and its row is not read.  Logits of -inf have
  * probability zero; a row without a finite logit, or with NaN or +inf, gives NaN.  stats (optional): [rows, 2] floats
- * for molt_token_logprob_bwd (max and log2 of the sum).  fp32 arithmetic. */
+ * for molt_token_logprob_bwd (what the exponents were taken from, and log2 of the sum).  fp32 arithmetic. */
 int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, float temperature,
                            float* logprob, float* stats, int64_t rows, int64_t vocab, uintptr_t stream);
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from array import array
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -256,6 +257,23 @@ def set_option(option: int, value: int) -> None:
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+_ITEM_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
+
+
+def grad_items(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]] = None) -> array:
+    """``molt_grad_item`` records (four 64-bit fields each) of a list of gradients and, when clipping, their outputs."""
+    flat = [0] * (4 * len(grads))
+    flat[0::4] = map(torch.Tensor.data_ptr, grads)
+    if outs is not None:
+        flat[1::4] = flat[0::4] if outs is grads else map(torch.Tensor.data_ptr, outs)
+    flat[2::4] = map(torch.Tensor.numel, grads)
+    try:
+        flat[3::4] = [_ITEM_DTYPES[t.dtype] for t in grads]
+    except KeyError:
+        raise CapabilityError("gradient norms support bfloat16 and float32 tensors") from None
+    return array("q", flat)
 
 
 def make_desc(packed: torch.Tensor, absmax: torch.Tensor, n: int, k: int, blocksize: int, nibble_order: int,

@@ -147,19 +147,35 @@ class ParamArena:
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), betas, float(eps), float(weight_decay)
         self.steps = 0
 
-    def step(self, grad_scale: float = 1.0) -> None:
-        """One AdamW step over every parameter, on the current stream."""
-        import ctypes  # noqa: F401  (the native binding passes raw pointers)
+    def step(self, grad_scale: float = 1.0, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
+        """One AdamW step over every parameter, on the current stream.
 
+        With ``max_norm`` the gradients (times ``grad_scale``) are clipped to that global norm inside the optimizer's pass:
+        one kernel more reads them for the norm, none rewrites them.  Returns the norm before clipping, a scalar on the
+        device (after a summing all-reduce every rank finds the same one); a step whose norm is not finite changes
+        neither parameters nor moments."""
         from molt_b200 import _native
 
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError("max_norm must not be negative")
         self.steps += 1
         flat = self.flat
+        arguments = [flat.data_ptr(), self.grads.flat.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                     flat.numel(), self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.steps,
+                     float(grad_scale)]
+        lib = _native.library()
         with torch.cuda.device(flat.device):
-            _native.check(_native.library().molt_adamw_step(
-                flat.data_ptr(), self.grads.flat.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                flat.numel(), self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.steps,
-                float(grad_scale), _native.stream_handle(flat.device)))
+            stream = _native.stream_handle(flat.device)
+            if max_norm is None:
+                _native.check(lib.molt_adamw_step(*arguments, stream))
+                return None
+            item = _native.grad_items((self.grads.flat,))
+            clip = torch.empty(2, dtype=torch.float32, device=flat.device)
+            scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(1), flat.device)
+            _native.check(lib.molt_grad_norm(item.buffer_info()[0], 1, _native.NORM_L2, float(grad_scale), float(max_norm),
+                                             clip.data_ptr(), scratch.data_ptr(), scratch.numel(), stream))
+            _native.check(lib.molt_adamw_step_clipped(*arguments, clip.data_ptr(), stream))
+        return clip[0]
 
 
 class RankLeftError(RuntimeError):

@@ -2,7 +2,6 @@
 backward pass and the optimizer step.  Nothing is read back to the host."""
 from __future__ import annotations
 
-from array import array
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -10,7 +9,6 @@ import torch
 from molt_b200 import _native
 from molt_b200.core.errors import CapabilityError
 
-_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
 _NORMS = {2.0: _native.NORM_L2, float("inf"): _native.NORM_MAX}
 
 Grads = Union[torch.Tensor, Sequence[torch.Tensor]]
@@ -43,27 +41,16 @@ def _norm_kind(norm_type: float) -> int:
     return kind
 
 
-def _items(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]]) -> array:
-    """The list as ``molt_grad_item`` records."""
+def _check_device(grads: Tuple[torch.Tensor, ...]) -> None:
     if grads[0].device.type != "cuda" or len(set(map(torch.Tensor.get_device, grads))) != 1:
         if any(t.device.type != "cuda" for t in grads):
             raise CapabilityError("gradient norms require CUDA tensors")
         raise ValueError("all gradients must be on one device")
-    try:
-        dtypes = [_DTYPES[t.dtype] for t in grads]
-    except KeyError:
-        raise CapabilityError("gradient norms support bfloat16 and float32 tensors") from None
-    flat = [0] * (4 * len(grads))
-    flat[0::4] = map(torch.Tensor.data_ptr, grads)
-    if outs is not None:
-        flat[1::4] = flat[0::4] if outs is grads else map(torch.Tensor.data_ptr, outs)
-    flat[2::4] = map(torch.Tensor.numel, grads)
-    flat[3::4] = dtypes
-    return array("q", flat)
 
 
 def _launch(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]], kind: int, max_norm: float) -> torch.Tensor:
-    items, device, count = _items(grads, outs), grads[0].device, len(grads)
+    _check_device(grads)
+    items, device, count = _native.grad_items(grads, outs), grads[0].device, len(grads)
     lib = _native.library()
     scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(count), device)
     result = torch.empty(2, dtype=torch.float32, device=device)

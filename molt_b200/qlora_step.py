@@ -22,6 +22,8 @@ from torch.nn import functional as F
 
 from molt_b200 import _native
 from molt_b200.data_parallel import GradArena, ParamArena, StepGuard, lora_parameters
+from molt_b200.kernels.policy_loss import clipped_policy_loss, preference_loss
+from molt_b200.kernels.token_logprobs import token_logprobs, token_logprobs_with_grad
 from molt_b200.methods._linear import LoraShadows, ShadowTable
 from molt_b200.methods.quant_state import NestedState, QuantState
 from molt_b200.modules import GatedMLP, NF4LoRALinear
@@ -332,6 +334,54 @@ class _FrozenHeadLoss(torch.autograd.Function):
         return grad * grad_output.to(grad.dtype), None, None, None, None
 
 
+class _FrozenHeadLogprobs(torch.autograd.Function):
+    """Token log-probabilities through a frozen bf16 LM head, in row chunks, without keeping the logits.  The gradient of
+    any loss with respect to a row of logits is (dLoss / dlogprob) times a row that the forward pass already knows, so the
+    forward turns the logits into that row in place and multiplies it by the head at once; what the backward pass has
+    left to do is to scale rows of the hidden width."""
+
+    @staticmethod
+    def forward(ctx, hidden, head, token_ids, chunk, temperature, trained):
+        hidden = hidden.contiguous()
+        rows, vocab = hidden.shape[0], head.shape[0]
+        native = hidden.dtype == torch.bfloat16 and head.dtype == torch.bfloat16 and vocab % 64 == 0 and hidden.shape[1] % 64 == 0
+        logprobs = torch.empty(rows, dtype=torch.float32, device=hidden.device)
+        unit = torch.empty_like(hidden) if trained else None
+        for start in range(0, rows, chunk):
+            part = slice(start, start + chunk)
+            logits = dense_gemm(head, hidden[part], False) if native else hidden[part] @ head.t()
+            if trained:
+                logprobs[part], logits = token_logprobs_with_grad(logits, token_ids[part], temperature=temperature, out=logits)
+                unit[part] = dense_gemm(head, logits, True) if native else logits @ head
+            else:
+                logprobs[part] = token_logprobs(logits, token_ids[part], temperature)
+        if trained:
+            ctx.save_for_backward(unit)
+        return logprobs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        (unit,) = ctx.saved_tensors
+        return (unit * grad_output[:, None]).to(unit.dtype), None, None, None, None, None
+
+
+def frozen_head_logprobs(hidden: torch.Tensor, head: torch.Tensor, token_ids: torch.Tensor, chunk: int = 8192,
+                         temperature: float = 1.0) -> torch.Tensor:
+    """``log_softmax(hidden @ head.T / temperature)`` at ``token_ids`` (fp32 ``[rows]``) for hidden states ``[rows, width]``
+    and a frozen head ``[vocab, width]``; differentiable with respect to the hidden states.  Two GEMMs per row chunk when a
+    gradient is wanted (the same number as for the cross-entropy of this head), one when it is not.  Ids outside the
+    vocabulary give 0 and no gradient."""
+    if head.requires_grad:
+        raise ValueError("the head must be frozen")
+    if hidden.dim() != 2 or head.dim() != 2 or hidden.shape[1] != head.shape[1] or token_ids.shape != hidden.shape[:1]:
+        raise ValueError("hidden must be [rows, width], head [vocab, width] and token_ids [rows]")
+    if chunk < 1:
+        raise ValueError("chunk must be positive")
+    trained = hidden.requires_grad and torch.is_grad_enabled()
+    return _FrozenHeadLogprobs.apply(hidden, head, token_ids, int(chunk), float(temperature), trained)
+
+
 class SyntheticDecoder(nn.Module):
     def __init__(self, shape: DecoderShape, device, seed: int = 1337, layers: Optional[int] = None):
         super().__init__()
@@ -350,10 +400,9 @@ class SyntheticDecoder(nn.Module):
         self.register_buffer("cos", angles.cos().bfloat16()[None, None], persistent=False)
         self.register_buffer("sin", angles.sin().bfloat16()[None, None], persistent=False)
 
-    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, global_tokens: int, replay_up: bool = True,
-             layer_done=None) -> torch.Tensor:
-        """``layer_done(index)``, when given, is called during backward as soon as layer ``index`` has produced all of
-        its adapter gradients (layers finish from the last to the first)."""
+    def hidden_states(self, tokens: torch.Tensor, replay_up: bool = True, layer_done=None) -> torch.Tensor:
+        """Final hidden states ``[batch * seq, hidden]``.  ``layer_done(index)``, when given, is called during backward as
+        soon as layer ``index`` has produced all of its adapter gradients (layers finish from the last to the first)."""
         stream, delta = F.embedding(tokens, self.embed).requires_grad_(), None
         for index, layer in enumerate(self.layers):
             hook = None
@@ -363,8 +412,69 @@ class SyntheticDecoder(nn.Module):
                     return grad
             stream, delta = layer.step(stream, delta, self.cos, self.sin, replay_up, hook)
         _, hidden = self.final_norm.add_and_norm(stream, delta)
-        hidden = hidden.reshape(-1, self.shape.hidden)
+        return hidden.reshape(-1, self.shape.hidden)
+
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, global_tokens: int, replay_up: bool = True,
+             layer_done=None) -> torch.Tensor:
+        """Cross-entropy summed over the tokens and divided by ``global_tokens``."""
+        hidden = self.hidden_states(tokens, replay_up, layer_done)
         return _FrozenHeadLoss.apply(hidden, self.head, targets.reshape(-1), self.head_chunk, float(global_tokens))
+
+    def logprobs(self, tokens: torch.Tensor, targets: torch.Tensor, replay_up: bool = True, layer_done=None,
+                 temperature: float = 1.0) -> torch.Tensor:
+        """Log-probability ``[batch, seq]`` of every target given the tokens up to its place."""
+        hidden = self.hidden_states(tokens, replay_up, layer_done)
+        return frozen_head_logprobs(hidden, self.head, targets.reshape(-1), self.head_chunk, temperature).view(targets.shape)
+
+
+@dataclass(frozen=True)
+class CrossEntropy:
+    """Next-token training: ``QLoRAStep.run(tokens, targets)``."""
+
+    def loss(self, model: SyntheticDecoder, world: int, layer_done, tokens, targets):
+        return model.loss(tokens, targets, model.shape.tokens * world, layer_done=layer_done)
+
+    def grad_scale(self, world: int) -> float:
+        return 1.0   # the loss is already normalised by the global token count
+
+
+@dataclass(frozen=True)
+class PolicyObjective:
+    """Policy tuning: ``QLoRAStep.run(tokens, targets, old_logprobs, advantages, mask, ref_logprobs)``, the last two
+    optional.  All but ``advantages`` (``[batch, seq]`` or ``[batch]``) are ``[batch, seq]``.  Ranks average their means."""
+
+    clip_low: float = 0.2
+    clip_high: float = 0.2
+    kl_coef: float = 0.0
+    reduction: str = "token"
+    temperature: float = 1.0
+
+    def loss(self, model: SyntheticDecoder, world: int, layer_done, tokens, targets, old_logprobs, advantages, mask=None,
+             ref_logprobs=None):
+        logprobs = model.logprobs(tokens, targets, layer_done=layer_done, temperature=self.temperature)
+        return clipped_policy_loss(logprobs, old_logprobs, advantages, mask, ref_logprobs, self.clip_low, self.clip_high,
+                                   self.kl_coef, self.reduction).loss
+
+    def grad_scale(self, world: int) -> float:
+        return 1.0 / world
+
+
+@dataclass(frozen=True)
+class PreferenceObjective:
+    """Preference tuning: ``QLoRAStep.run(tokens, targets, mask, ref_logprobs)``, both optional, with the chosen sequences in
+    the first half of the batch and the rejected ones in the second.  Ranks average their means."""
+
+    beta: float = 0.1
+    label_smoothing: float = 0.0
+    kind: str = "sigmoid"
+    average: bool = False
+
+    def loss(self, model: SyntheticDecoder, world: int, layer_done, tokens, targets, mask=None, ref_logprobs=None):
+        logprobs = model.logprobs(tokens, targets, layer_done=layer_done)
+        return preference_loss(logprobs, ref_logprobs, mask, self.beta, self.label_smoothing, self.kind, self.average).loss
+
+    def grad_scale(self, world: int) -> float:
+        return 1.0 / world
 
 
 def attach_lora_shadows(model: nn.Module) -> list:
@@ -382,7 +492,10 @@ def attach_lora_shadows(model: nn.Module) -> list:
 
 
 class QLoRAStep:
-    """Holds model, gradient arena and optimiser; ``run(tokens, targets)`` is one data-parallel training step.
+    """Holds model, gradient arena and optimiser; ``run(tokens, targets)`` is one data-parallel training step on the
+    cross-entropy, or with another ``objective`` (:class:`PolicyObjective`, :class:`PreferenceObjective`) ``run`` takes that
+    one's inputs.  ``max_grad_norm`` clips the global gradient norm inside the optimizer's pass; ``grad_norm`` then holds the
+    last step's norm on the device.
 
     Step anatomy: zero the gradient arena; forward; backward, during which every decoder layer's bucket of the arena
     goes to the all-reduce (side stream) as soon as the layer's backward has run, so the exchange overlaps the backward
@@ -393,7 +506,9 @@ class QLoRAStep:
 
     def __init__(self, shape: DecoderShape, device, layers: Optional[int] = None, lr: float = 1e-4,
                  cuda_graph: bool = False, status_interval: int = 50, guard: Optional[StepGuard] = None,
-                 lora_shadows: bool = True):
+                 lora_shadows: bool = True, objective=None, max_grad_norm: Optional[float] = None):
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError("max_grad_norm must not be negative")
         self.shape = shape
         self.device = device
         self.world = dist.get_world_size() if dist.is_initialized() else 1
@@ -413,9 +528,13 @@ class QLoRAStep:
         self.cuda_graph = cuda_graph
         self.status_interval = int(status_interval)
         self.guard = guard
+        self.objective = CrossEntropy() if objective is None else objective
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
         self.steps = 0
         self._graph: Optional[torch.cuda.CUDAGraph] = None
-        self._static_tokens = self._static_targets = self._static_loss = None
+        self._static_inputs: tuple = ()
+        self._static_loss = None
         self._eager_steps = 0
         self.graph_launches = 0      # library kernel launches recorded in the CUDA graph
         self.replayed_launches = 0   # library kernel launches executed through graph replays so far
@@ -424,41 +543,48 @@ class QLoRAStep:
         if self.world > 1:
             self.arena.all_reduce_bucket(self.layer_bucket[index])
 
-    def _forward_backward(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def _forward_backward(self, *inputs) -> torch.Tensor:
         self.arena.zero()
-        loss = self.model.loss(tokens, targets, self.shape.tokens * self.world,
-                               layer_done=self._layer_done if self.world > 1 else None)
+        loss = self.objective.loss(self.model, self.world, self._layer_done if self.world > 1 else None, *inputs)
         loss.backward()
         self.arena.wait()            # the current stream joins the collectives issued from the backward
         return loss.detach()
 
-    def _capture(self, tokens: torch.Tensor, targets: torch.Tensor) -> None:
+    def _capture(self, *inputs) -> None:
         """Record forward + backward (+ the overlapped collectives) of one micro-batch once; every later step replays
         the recording (the kernels take raw pointers and never allocate or synchronise, so they are capture-safe)."""
-        self._static_tokens = tokens.clone()
-        self._static_targets = targets.clone()
+        self._static_inputs = tuple(None if t is None else t.clone() for t in inputs)
         self._graph = torch.cuda.CUDAGraph()
         lib = _native.library()
         before = lib.molt_launch_count()
         with torch.cuda.graph(self._graph):
-            self._static_loss = self._forward_backward(self._static_tokens, self._static_targets)
+            self._static_loss = self._forward_backward(*self._static_inputs)
         self.graph_launches = int(lib.molt_launch_count() - before)   # library kernels recorded; each replay runs them
 
-    def run(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def _stage(self, *inputs) -> None:
+        shapes = [None if t is None else t.shape for t in inputs]
+        if shapes != [None if held is None else held.shape for held in self._static_inputs]:
+            raise ValueError("the inputs of a captured step keep their number and shapes")
+        for t, held in zip(inputs, self._static_inputs):
+            if t is not None:
+                held.copy_(t)
+
+    def run(self, *inputs: Optional[torch.Tensor]) -> torch.Tensor:
         if self.guard is not None:
             self.guard.check(self.steps)     # host-side: every peer is alive and about to run the same step
         if self.cuda_graph and self._graph is None and self._eager_steps >= 2:
-            self._capture(tokens, targets)
+            self._capture(*inputs)
         if self._graph is not None:
-            self._static_tokens.copy_(tokens)
-            self._static_targets.copy_(targets)
+            self._stage(*inputs)
             self._graph.replay()
             self.replayed_launches += self.graph_launches
             loss = self._static_loss
         else:
-            loss = self._forward_backward(tokens, targets)
+            loss = self._forward_backward(*inputs)
             self._eager_steps += 1
-        self.optimizer.step(grad_scale=1.0)  # the loss is already normalised by the global token count
+        norm = self.optimizer.step(grad_scale=self.objective.grad_scale(self.world), max_norm=self.max_grad_norm)
+        if norm is not None:
+            self.grad_norm = norm
         if self.shadows is not None:
             self.shadows.refresh()           # same stream, behind the step: the next forward sees the new adapters
         self.steps += 1

@@ -190,3 +190,22 @@ def test_host_tensors_are_refused(native_library):
         kernels.clip_grad_norm([lp], -1.0)
     with pytest.raises(ValueError):
         kernels.global_grad_norm([torch.zeros(4, 4)[:, :2]])
+
+
+def test_step_driver_arguments_are_checked_on_the_host():
+    from molt_b200.data_parallel import GradArena, ParamArena
+    from molt_b200.qlora_step import CrossEntropy, PolicyObjective, PreferenceObjective, QLoRAStep, LLAMA3_8B, frozen_head_logprobs
+
+    with pytest.raises(ValueError):
+        QLoRAStep(LLAMA3_8B, torch.device("cpu"), max_grad_norm=-1.0)
+    state = ParamArena(GradArena([torch.nn.Parameter(torch.zeros(4))]))
+    with pytest.raises(ValueError):
+        state.step(max_norm=float("nan"))
+    assert state.steps == 0
+    assert [o.grad_scale(4) for o in (CrossEntropy(), PolicyObjective(), PreferenceObjective())] == [1.0, 0.25, 0.25]
+    hidden, head, ids = torch.zeros(3, 8), torch.zeros(16, 8), torch.zeros(3, dtype=torch.int64)
+    for bad in ((hidden[0], head, ids), (hidden, head[:, :4], ids), (hidden, head, ids[:2])):
+        with pytest.raises(ValueError):
+            frozen_head_logprobs(*bad)
+    with pytest.raises(CapabilityError):
+        frozen_head_logprobs(hidden, head, ids)
