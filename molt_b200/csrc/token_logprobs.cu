@@ -63,15 +63,18 @@ struct Vec<float> {
   static __device__ __forceinline__ float largest(const uint4& q, float m) {
     return fmaxf(fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w))), m);
   }
+  // f of every pair of differences x - m
   template <typename F>
-  static __device__ __forceinline__ void each(const uint4& q, F f) {
-    f(0, pair(__uint_as_float(q.x), __uint_as_float(q.y)));
-    f(1, pair(__uint_as_float(q.z), __uint_as_float(q.w)));
+  static __device__ __forceinline__ void each(const uint4& q, float m, F f) {
+    const pair_t minus = pair(-m, -m);
+    f(add2(pair(__uint_as_float(q.x), __uint_as_float(q.y)), minus));
+    f(add2(pair(__uint_as_float(q.z), __uint_as_float(q.w)), minus));
   }
   template <typename F>
-  static __device__ __forceinline__ uint4 map(const uint4& q, F f) {
-    const float2 a = halves(f(pair(__uint_as_float(q.x), __uint_as_float(q.y))));
-    const float2 b = halves(f(pair(__uint_as_float(q.z), __uint_as_float(q.w))));
+  static __device__ __forceinline__ uint4 map(const uint4& q, float m, F f) {
+    const pair_t minus = pair(-m, -m);
+    const float2 a = halves(f(add2(pair(__uint_as_float(q.x), __uint_as_float(q.y)), minus)));
+    const float2 b = halves(f(add2(pair(__uint_as_float(q.z), __uint_as_float(q.w)), minus)));
     return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
   }
 };
@@ -88,19 +91,26 @@ struct Vec<__nv_bfloat16> {
     const unsigned v = max2(max2(q.x, q.y), max2(q.z, q.w));
     return fmaxf(m, fmaxf(bf16_lo(v), bf16_hi(v)));
   }
-  template <typename F>
-  static __device__ __forceinline__ void each(const uint4& q, F f) {
-    const unsigned w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f(i, pair(bf16_lo(w[i]), bf16_hi(w[i])));
+  // x - m in fp32 straight from the bf16 halves of a word, one instruction each
+  static __device__ __forceinline__ pair_t differences(unsigned w, float m) {
+    float a, b;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tsub.rn.f32.bf16 %0, lo, %3;\n\tsub.rn.f32.bf16 %1, hi, %3;\n\t}"
+        : "=f"(a), "=f"(b) : "r"(w), "f"(m));
+    return pair(a, b);
   }
   template <typename F>
-  static __device__ __forceinline__ uint4 map(const uint4& q, F f) {
+  static __device__ __forceinline__ void each(const uint4& q, float m, F f) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f(differences(w[i], m));
+  }
+  template <typename F>
+  static __device__ __forceinline__ uint4 map(const uint4& q, float m, F f) {
     const unsigned w[4] = {q.x, q.y, q.z, q.w};
     unsigned o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 h = halves(f(pair(bf16_lo(w[i]), bf16_hi(w[i]))));
+      const float2 h = halves(f(differences(w[i], m)));
       o[i] = pack_bf16x2(h.x, h.y);
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
@@ -128,11 +138,23 @@ struct Running {
 #pragma unroll
     for (int j = 0; j < N; ++j) top = Vec<T>::largest(q[j], top);
     raise(top);
-    const float from = -base();
-    const pair_t minus = pair(from, from), cc = pair(c, c);
+    const float from = base();
+    const pair_t cc = pair(c, c);
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      Vec<T>::each(q[j], [&](int, pair_t x) { s = add2(s, exp2_2(mul2(add2(x, minus), cc))); });
+    for (int j = 0; j < N; ++j) Vec<T>::each(q[j], from, [&](pair_t d) { s = add2(s, exp2_2(mul2(d, cc))); });
+  }
+  // The same with a reference that stays until a batch exceeds it by 2^8: sums stay far from fp32's limits, ln s (whose
+  // rounding stays in the result) stays small, and the rescaling is hardly ever executed.
+  template <typename T, int N>
+  __device__ __forceinline__ void take_lazily(const uint4 (&q)[N]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = Vec<T>::largest(q[j], top);
+    if (top > m + 8.f / c) raise(top);
+    const float from = base();
+    const pair_t cc = pair(c, c);
+#pragma unroll
+    for (int j = 0; j < N; ++j) Vec<T>::each(q[j], from, [&](pair_t d) { s = add2(s, exp2_2(mul2(d, cc))); });
   }
   __device__ __forceinline__ void take_one(float x) {
     raise(fmaxf(m, x));
@@ -298,101 +320,140 @@ __device__ __forceinline__ void copy_wait() {
 // once) and by latency in practice, since no gradient can be formed before the whole row has been seen.  A row does not fit
 // one SM (151936 bf16 logits are 304 KB), so a cluster of blocks shares it, and the second pass reads it again from the L2:
 // 5 blocks of 256 threads per SM, at most 20 vectors per thread, keep 60 MB of rows in flight.  What keeps the loads going is
-// a ring of RING batches of B vectors per thread in shared memory, filled by asynchronous copies that each thread makes for
-// itself (no barrier): the first pass runs it upwards, the second one downwards, beginning with the batches that it still
-// holds.  2048 rows of 151936 bf16: 212 us (5.9 TB/s of 6.55).  Other forms, same rows: loads through registers 232, rows
-// held in the registers of a cluster 291-388, in its shared memory 253-390 (the join of the row then leaves the memory
-// idle), persistent blocks that fetch their next row early 231-296, two kernels (forward, then backward_kernel) 280.
+// a ring of kRing batches of kRingBatch vectors per thread in shared memory, filled by asynchronous copies that each thread
+// makes for itself (no barrier): the first pass runs it upwards, the second one downwards, beginning with the batches that
+// it still holds.  The ring is unrolled and the cluster's size a constant, so that a batch of 16 elements costs few
+// instructions beside its arithmetic (27 per pair of elements in all; 38 with computed slots and addresses, which took
+// 225 us and drew more power).  2048 rows of 151936 bf16: 212 us, 205 in place, where a copy of the same bytes takes 195;
+// 8192 rows 0.81 ms, and 0.88-0.91 in a long loop, when the power cap lowers the clock.  Other forms, same 2048 rows: loads
+// through registers 232 us, rows held in the registers of a cluster 291-388, in its shared memory 253-390 (the join of the
+// row then leaves the memory idle), persistent blocks that fetch their next row early 231-296, two kernels (forward, then
+// backward_kernel) 280.
 constexpr int kRing = 5, kRingBatch = 2;
 
-template <typename T, int THREADS, int BLOCKS>
+template <typename T, int THREADS, int CLUSTER, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
     row_grad_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids, const float* __restrict__ weight,
                     float inv_t, float* __restrict__ logprob, T* grad, long long grad_stride, int vocab) {
-  constexpr int E = Vec<T>::kElements, B = kRingBatch;
-  extern __shared__ uint4 ring[];   // [kRing * B][THREADS]
-  const unsigned size = cluster_size(), rank = cluster_rank();
-  const long long row = blockIdx.x / size, t = ids[row];
+  constexpr int E = Vec<T>::kElements, B = kRingBatch, R = kRing, kStep = CLUSTER * THREADS, kBatch = B * kStep;
+  extern __shared__ uint4 ring[];   // [R * B][THREADS]
+  const unsigned rank = CLUSTER > 1 ? cluster_rank() : 0;
+  const long long row = blockIdx.x / CLUSTER, t = ids[row];
   const T* x = logits + row * row_stride;
   T* g = grad + row * grad_stride;
-  const int first = rank * THREADS + threadIdx.x, step = size * THREADS;
+  const int first = rank * THREADS + threadIdx.x;
   if (t < 0 || t >= vocab) {
     if (first == 0) logprob[row] = 0.f;
-    clear(g, 0, vocab, first, step);
+    clear(g, 0, vocab, first, kStep);
     return;
   }
-  if (size > 1) cluster_arrive();
+  if (CLUSTER > 1) cluster_arrive();
   const Cut<T> cut(x, vocab);
-  const uint4* p = reinterpret_cast<const uint4*>(x + cut.head);
-  uint4* mine = ring + threadIdx.x;
-  const int batches = ((cut.vectors + step - 1) / step + B - 1) / B;   // the same for every thread of the row
-  const auto fetch = [&](int k, int slot) {
+  // batches of B vectors per thread: `whole` that every thread has in full, and one more where some vectors are missing
+  const int whole = cut.vectors / kBatch, left = cut.vectors - whole * kBatch;
+  const uint4* from = reinterpret_cast<const uint4*>(x + cut.head) + first;   // the next batch to be fetched
+  uint4* const mine = ring + threadIdx.x;
+  const auto fetch = [&](int r) {
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      const int v = first + (k * B + j) * step;
-      if (v < cut.vectors) copy_async(mine + (slot * B + j) * THREADS, p + v);
-    }
+    for (int j = 0; j < B; ++j) copy_async(mine + (r * B + j) * THREADS, from + j * kStep);
+  };
+  const auto fetch_partial = [&](int r) {
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (first + j * kStep < left) copy_async(mine + (r * B + j) * THREADS, from + j * kStep);
   };
 #pragma unroll
-  for (int k = 0; k < kRing; ++k) {
-    if (k < batches) fetch(k, k);
+  for (int r = 0; r < R; ++r) {
+    if (r < whole) fetch(r);
+    else if (r == whole) fetch_partial(r);
     copy_commit();
+    from += kBatch;
   }
   const int loose = first < 16 ? cut.loose(first, vocab) : -1;
   const float loose_x = loose >= 0 ? load1(x + loose) : 0.f;
+  const float xt = load1(x + t);   // by all: before any of it may be overwritten
   const float w = (weight != nullptr ? weight[row] : 1.f) * inv_t;
   Running run;
   run.c = inv_t * kLog2e;
-  int slot = 0;
-  for (int k = 0; k < batches; ++k) {
-    copy_wait<kRing - 1>();
+  const auto take = [&](int r) {
+    copy_wait<R - 1>();
     uint4 q[B];
 #pragma unroll
-    for (int j = 0; j < B; ++j)
-      q[j] = first + (k * B + j) * step < cut.vectors
-                 ? mine[(slot * B + j) * THREADS]
-                 : make_uint4(Vec<T>::kMinusInf, Vec<T>::kMinusInf, Vec<T>::kMinusInf, Vec<T>::kMinusInf);
-    run.template take<T, B>(q);
-    if (k + kRing < batches) fetch(k + kRing, slot);   // into the slot that has just been read
-    copy_commit();
-    slot = slot + 1 == kRing ? 0 : slot + 1;
+    for (int j = 0; j < B; ++j) q[j] = mine[(r * B + j) * THREADS];
+    run.template take_lazily<T, B>(q);
+  };
+  int k = 0;
+  for (; k + R <= whole; k += R) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      take(r);
+      if (k + r + R < whole) fetch(r);   // into the slot that has just been read
+      else if (k + r + R == whole) fetch_partial(r);
+      copy_commit();
+      from += kBatch;
+    }
+  }
+  const int rest = whole - k;   // batches behind the last full round of the ring; the partial one is number `rest` of this round
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r < rest) {
+      take(r);
+      copy_commit();
+    } else if (r == rest && left > 0) {
+      copy_wait<0>();
+#pragma unroll
+      for (int j = 0; j < B; ++j)
+        if (first + j * kStep < left) {
+          const uint4 q[1] = {mine[(r * B + j) * THREADS]};
+          run.template take_lazily<T, 1>(q);
+        }
+    }
   }
   if (loose >= 0) run.take_one(loose_x);
   const float2 sums = halves(run.s);
   float m = run.m, s = sums.x + sums.y;
-  row_join<THREADS>(m, s, run.c, rank, size);
+  row_join<THREADS>(m, s, run.c, rank, CLUSTER);
   const float log2_s = log2f(s);
-  const pair_t minus = pair(-m, -m), cc = pair(run.c, run.c), less = pair(-log2_s, -log2_s), scale = pair(-w, -w);
-  const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
-  // the target's own column, by the thread that holds it: 1 - p without the cancellation
-  const auto target = [&](float xt) {
-    const float l = (xt - m) * inv_t - log2_s * kLn2;
-    logprob[row] = l;
-    store1(g + t, -expm1f(l) * w);
-  };
+  const float l = (xt - m) * inv_t - log2_s * kLn2;
+  if (first == 0) logprob[row] = l;
+  const pair_t cc = pair(run.c, run.c), less = pair(-log2_s, -log2_s), scale = pair(-w, -w);
+  const auto f = [&](pair_t d) { return mul2(exp2_2(fma2(d, cc, less)), scale); };
   const bool alike = cut_alike(x, g);
-  const int at = (int)t - cut.head;
-  const int holder = at >= 0 && at / E < cut.vectors ? at / E : -1;
-  T* to = g + cut.head;
-  for (int k = batches - 1; k >= 0; --k) {
-    slot = slot == 0 ? kRing - 1 : slot - 1;
-    copy_wait<kRing - 1>();
+  const long long behind = (long long)whole * kBatch;
+  T* to = g + cut.head + (behind + first) * E;                                                      // the batch given next
+  from = reinterpret_cast<const uint4*>(x + cut.head) + first + (behind - (long long)R * kBatch);   // R batches before it
+  const auto give = [&](int r, int j) { put(to + j * (kStep * E), Vec<T>::map(mine[(r * B + j) * THREADS], m, f), alike); };
+  const auto give_batch = [&](int r) {
+    to -= kBatch * E;
+    from -= kBatch;
+    copy_wait<R - 1>();
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      const int v = first + (k * B + j) * step;
-      if (v < cut.vectors) {
-        const uint4* held = mine + (slot * B + j) * THREADS;
-        put(to + (long long)v * E, Vec<T>::map(*held, f), alike);
-        if (v == holder) target(load1(reinterpret_cast<const T*>(held) + (at - v * E)));
-      }
-    }
-    if (k >= kRing) fetch(k - kRing, slot);
+    for (int j = 0; j < B; ++j) give(r, j);
+    if (k > 0) fetch(r);
     copy_commit();
+  };
+  copy_wait<0>();
+#pragma unroll
+  for (int r = R - 1; r >= 0; --r) {
+    if (r < rest) {
+      give_batch(r);
+    } else if (r == rest && left > 0) {
+#pragma unroll
+      for (int j = 0; j < B; ++j)
+        if (first + j * kStep < left) give(r, j);
+      if (k > 0) fetch(r);
+      copy_commit();
+    }
   }
-  if (loose >= 0) {
-    if (loose == (int)t) target(loose_x);
-    else store1(g + loose, exp2_fast((loose_x - m) * run.c - log2_s) * -w);
+  for (k -= R; k >= 0; k -= R) {
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) give_batch(r);
   }
+  if (loose >= 0) store1(g + loose, exp2_fast((loose_x - m) * run.c - log2_s) * -w);
+  // the target's own column, by the thread that has just written it: 1 - p without the cancellation
+  const int at = (int)t - cut.head;
+  const bool own = at >= 0 && at / E < cut.vectors ? at / E % kStep == first : loose == (int)t;
+  if (own) store1(g + t, -expm1f(l) * w);
 }
 
 // A block takes 4 vectors per thread of one row: no loop, many blocks, reads and writes spread evenly.
@@ -424,8 +485,8 @@ __global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits,
     if (first + j * kBackThreads < end) q[j] = __ldcs(p + first + j * kBackThreads);
   const float c = inv_t * kLog2e, w = grad_logprob[row] * inv_t;
   const float2 st = stats[row];
-  const pair_t minus = pair(-st.x, -st.x), cc = pair(c, c), less = pair(-st.y, -st.y), scale = pair(-w, -w);
-  const auto f = [&](pair_t a) { return mul2(exp2_2(fma2(add2(a, minus), cc, less)), scale); };
+  const pair_t cc = pair(c, c), less = pair(-st.y, -st.y), scale = pair(-w, -w);
+  const auto f = [&](pair_t d) { return mul2(exp2_2(fma2(d, cc, less)), scale); };
   const bool alike = cut_alike(x, g);
   const int at = (int)t - cut.head, holder = at / E;
   const bool inside = at >= 0 && holder < cut.vectors;
@@ -435,7 +496,7 @@ __global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits,
     if (v < end) {
       const bool own = inside && v == holder;
       const float xt = own ? load1(x + t) : 0.f;   // before it may be overwritten
-      put(g + cut.head + (long long)v * E, Vec<T>::map(q[j], f), alike);
+      put(g + cut.head + (long long)v * E, Vec<T>::map(q[j], st.x, f), alike);
       if (own) store1(g + t, -expm1f((xt - st.x) * inv_t - st.y * kLn2) * w);
     }
   }
@@ -529,13 +590,17 @@ int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, cons
   auto* x = reinterpret_cast<const T*>(logits);
   auto* id = reinterpret_cast<const long long*>(ids);
   auto* g = reinterpret_cast<T*>(grad);
-  if (vectors <= 64 * 8)
-    return launch_clusters("token_logprob row_grad_kernel", row_grad_kernel<T, 64, 16>, rows, 1, 64, 64 * kSlots, s, x, row_stride, id,
-                           weight, 1.f / temperature, logprob, g, grad_stride, vocab);
+  const auto launch = [&](auto kernel, int cluster, int threads) {
+    return launch_clusters("token_logprob row_grad_kernel", kernel, rows, cluster, threads, threads * kSlots, s, x, row_stride, id, weight,
+                           1.f / temperature, logprob, g, grad_stride, vocab);
+  };
+  if (vectors <= 64 * 8) return launch(row_grad_kernel<T, 64, 1, 16>, 1, 64);
   int cluster = 1;
   while (cluster < 8 && (vectors > cluster * 256 * 20 || (rows * cluster < 148 * 4 && vectors >= cluster * 256 * 4))) cluster *= 2;
-  return launch_clusters("token_logprob row_grad_kernel", row_grad_kernel<T, 256, 5>, rows, cluster, 256, 256 * kSlots, s, x, row_stride, id,
-                         weight, 1.f / temperature, logprob, g, grad_stride, vocab);
+  if (cluster == 1) return launch(row_grad_kernel<T, 256, 1, 5>, 1, 256);
+  if (cluster == 2) return launch(row_grad_kernel<T, 256, 2, 5>, 2, 256);
+  if (cluster == 4) return launch(row_grad_kernel<T, 256, 4, 5>, 4, 256);
+  return launch(row_grad_kernel<T, 256, 8, 5>, 8, 256);
 }
 
 }  // namespace
