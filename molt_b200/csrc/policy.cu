@@ -4,6 +4,8 @@
 // pass, so the forward writes the gradient without either and the backward multiplies both in.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace molt {
@@ -11,33 +13,70 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Sum over a block in a fixed order; the result is valid in thread 0.
+// Sums of one thread: N in 64 bits, and M counts.
+template <int N, int M>
+struct Sums {
+  double v[N] = {};
+  int n[M] = {};
+
+  // Sums of the warp, in lane 0.
+  __device__ __forceinline__ void join_warp() {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
+#pragma unroll
+    for (int i = 0; i < M; ++i) n[i] = __reduce_add_sync(~0u, n[i]);
+  }
+  // Lane 0's sums as N + M doubles.
+  __device__ __forceinline__ void store(double* to, int stride) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i * stride] = v[i];
+#pragma unroll
+    for (int i = 0; i < M; ++i) to[(N + i) * stride] = n[i];
+  }
+};
+
+// Adds up, over a block and in a fixed order, what `store` left of every warp in part[value][warp]; thread i returns value i.
+__device__ __forceinline__ double join_block(const double* part, int values) {
+  __syncthreads();
+  double sum = 0.;
+  if (threadIdx.x < values)
+    for (int w = 0; w < (blockDim.x >> 5); ++w) sum += part[threadIdx.x * 32 + w];
+  return sum;
+}
+
+// Sum over a block in a fixed order, for all its threads.
 template <int N>
 __device__ __forceinline__ void block_sum(double (&v)[N]) {
-  __shared__ double part[N][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
-    if (lane == 0) part[i][warp] = v[i];
-  }
+  __shared__ double part[N * 32], total[N];
+  Sums<N, 1> sums;
+  for (int i = 0; i < N; ++i) sums.v[i] = v[i];
+  sums.join_warp();
+  if ((threadIdx.x & 31) == 0)
+    for (int i = 0; i < N; ++i) part[i * 32 + (threadIdx.x >> 5)] = sums.v[i];
+  const double mine = join_block(part, N);
+  if (threadIdx.x < N) total[threadIdx.x] = mine;
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int i = 0; i < N; ++i) {
-      double sum = 0.;
-      for (int w = 0; w < warps; ++w) sum += part[i][w];
-      v[i] = sum;
-    }
+  for (int i = 0; i < N; ++i) v[i] = total[i];
   __syncthreads();
 }
 
-// Tokens of a row one block takes: a row is cut when there are fewer rows than the device has room for blocks.
+using Full = std::integral_constant<bool, true>;
+using Ragged = std::integral_constant<bool, false>;
+
+constexpr int kUnroll = 4;                      // tokens a thread loads at a time
+constexpr int kRound = kThreads * kUnroll;      // tokens a block loads at a time
+
+// A row is cut where there are fewer rows than the device has room for blocks, into parts of whole rounds (so that no
+// block ends on a round that is mostly empty).  Fixed figures: the cut decides the order of the sums.
+int part_tokens(int64_t rows, int64_t seq) {
+  const int64_t want = (148 * 8 + rows - 1) / rows, even = (seq + want - 1) / want;
+  return (int)(even <= kRound ? kRound : even / kRound * kRound);
+}
 int splits_for(int64_t rows, int64_t seq) {
-  const int64_t most = (seq + kThreads * 4 - 1) / (kThreads * 4);
-  int64_t want = ((int64_t)148 * 8 + rows - 1) / rows;   // a fixed figure: the split decides the order of the sums
-  if (want > most) want = most;
-  return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
+  const int64_t per = part_tokens(rows, seq), splits = (seq + per - 1) / per;
+  return (int)(splits < 1 ? 1 : splits);
 }
 
 // A batch this small is one block's work: its row sums stay in shared memory and one launch gives the loss (4 x 64 tokens,
@@ -52,87 +91,91 @@ struct PolicyArgs {
   const float *logprob, *old, *ref, *advantage;
   const uint8_t* mask;
   long long lp_stride, old_stride, ref_stride, adv_stride, mask_stride;
-  long long batch, seq;
-  int per_token, splits;
+  long long batch;
+  int seq, per_token, splits, part;   // part: tokens of one of the splits of a row
   double log_high, log_low;   // ln(1 + clip_high), ln(1 - clip_low): the borders of ln r
   float log_high_f, log_low_f, high, low, kl_coef;   // the borders rounded to fp32; 1 + clip_high, 1 - clip_low
 };
 
-// exp(d) - 1 - d without the cancellation: the Taylor series d^2/2 (1 + d/3 (1 + d/4 (...))) where |d| is small (its
-// truncation is below 2^-26 relative for |d| <= 0.5 with ten terms), the plain difference elsewhere.
+// exp(d) - 1 - d without the cancellation: the Taylor series d^2 (1/2! + d (1/3! + d (1/4! + ...))) for |d| <= 1, to the term
+// d^12 (what it leaves out is below 2/13! < 2^-31 of the result), the plain difference elsewhere.  One range for nearly all
+// tokens of a policy near its reference, so that a warp seldom takes both ways.
 __device__ __forceinline__ float exp_minus_1_minus(float d) {
   if (d > 60.f) return expf(d);   // 1 + d is below its last bit; an infinite d must not meet itself
-  if (fabsf(d) > 0.5f) return expm1f(d) - d;
-  float r = 1.f;
+  if (fabsf(d) > 1.f) return expm1f(d) - d;
+  constexpr float kInverseFactorial[] = {1.f / 2, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320, 1.f / 362880,
+                                         1.f / 3628800, 1.f / 39916800, 1.f / 479001600};
+  float r = kInverseFactorial[10];
 #pragma unroll
-  for (int k = 10; k >= 3; --k) r = fmaf(r, d * (1.f / k), 1.f);
-  return 0.5f * d * d * r;
+  for (int k = 9; k >= 0; --k) r = fmaf(r, d, kInverseFactorial[k]);
+  return d * d * r;
 }
 
-// Tokens begin, begin + step, ... below end of row b, kUnroll of them loaded at a time.
-constexpr int kUnroll = 4;
-
-__device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, long long begin, long long end, int step,
-                                              float* __restrict__ unit_grad, double (&sum)[4]) {
-  for (long long t0 = begin; t0 < end; t0 += kUnroll * step) {
+// Tokens begin, begin + step, ... below end of row b, kUnroll of them loaded at a time; full rounds need no bounds checks.
+template <bool REF, bool MASK>
+__device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, int begin, int end, int step,
+                                              float* __restrict__ unit_grad, Sums<2, 2>& sum) {
+  const float* lp_row = a.logprob + b * a.lp_stride;
+  const float* old_row = a.old + b * a.old_stride;
+  const float* ref_row = REF ? a.ref + b * a.ref_stride : nullptr;
+  const uint8_t* mask_row = MASK ? a.mask + b * a.mask_stride : nullptr;
+  const float* adv_row = a.advantage + b * a.adv_stride;
+  const float one_adv = !a.per_token && begin < end ? adv_row[0] : 0.f;
+  float* unit_row = unit_grad != nullptr ? unit_grad + b * a.seq : nullptr;
+  const auto round = [&](int t0, auto full) {
+    constexpr bool FULL = decltype(full)::value;
     float lp[kUnroll], old[kUnroll], adv[kUnroll], ref[kUnroll];
     bool kept[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long t = t0 + j * step;
-      kept[j] = t < end;
-      if (kept[j]) {
-        lp[j] = a.logprob[b * a.lp_stride + t];
-        old[j] = a.old[b * a.old_stride + t];
-        adv[j] = a.advantage[b * a.adv_stride + (a.per_token ? t : 0)];
-        ref[j] = a.ref != nullptr ? a.ref[b * a.ref_stride + t] : 0.f;
-        kept[j] = a.mask == nullptr || a.mask[b * a.mask_stride + t] != 0;
-      }
+      const int t = FULL || t0 + j * step < end ? t0 + j * step : t0;   // a token of the row in any case
+      lp[j] = lp_row[t];
+      old[j] = old_row[t];
+      adv[j] = a.per_token ? adv_row[t] : one_adv;
+      if (REF) ref[j] = ref_row[t];
+      kept[j] = (FULL || t0 + j * step < end) && (!MASK || mask_row[t] != 0);
     }
     float loss = 0.f, ks = 0.f;
     int cuts = 0, keeps = 0;
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      float g = 0.f;
-      if (kept[j]) {
-        // fp32 rounds monotonously, so the rounded difference decides the border unless it lies on it
-        const float d = lp[j] - old[j];
-        bool cut = (adv[j] > 0.f && d > a.log_high_f) || (adv[j] < 0.f && d < a.log_low_f);
-        if (d == a.log_high_f || d == a.log_low_f) {
-          const double exact = (double)lp[j] - (double)old[j];
-          cut = (adv[j] > 0.f && exact > a.log_high) || (adv[j] < 0.f && exact < a.log_low);
-        }
-        float l = 0.f;
-        if (adv[j] != 0.f) {   // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
-          const float r = expf(d);
-          l = -(cut ? (adv[j] > 0.f ? a.high : a.low) : r) * adv[j];
-          g = cut ? 0.f : -r * adv[j];
-        }
-        if (a.ref != nullptr) {
-          const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
-          l += a.kl_coef * k;
-          g -= a.kl_coef * (k + e);   // exp(e) - 1
-          ks += k;
-        }
-        loss += l;
-        cuts += cut;
-        ++keeps;
+      // fp32 rounds monotonously, so the rounded difference decides the border unless it lies on it
+      const float d = lp[j] - old[j];
+      bool cut = (adv[j] > 0.f && d > a.log_high_f) || (adv[j] < 0.f && d < a.log_low_f);
+      if (d == a.log_high_f || d == a.log_low_f) {
+        const double exact = (double)lp[j] - (double)old[j];
+        cut = (adv[j] > 0.f && exact > a.log_high) || (adv[j] < 0.f && exact < a.log_low);
       }
-      if (unit_grad != nullptr && t0 + j * step < end) unit_grad[b * a.seq + t0 + j * step] = g;
+      const float r = expf(d);
+      // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
+      float l = adv[j] == 0.f ? 0.f : -(cut ? (adv[j] > 0.f ? a.high : a.low) : r) * adv[j];
+      float g = cut || adv[j] == 0.f ? 0.f : -r * adv[j];
+      if (REF) {
+        const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
+        l += a.kl_coef * k;
+        g -= a.kl_coef * (k + e);   // exp(e) - 1
+        ks += kept[j] ? k : 0.f;
+      }
+      loss += kept[j] ? l : 0.f;
+      cuts += kept[j] && cut;
+      keeps += kept[j];
+      if (unit_row != nullptr && (FULL || t0 + j * step < end)) unit_row[t0 + j * step] = kept[j] ? g : 0.f;
     }
     // four tokens in fp32, then in 64 bits: three roundings more on values that carry a few already
-    sum[0] += loss;
-    sum[1] += ks;
-    sum[2] += cuts;
-    sum[3] += keeps;
-  }
+    sum.v[0] += loss;
+    if (REF) sum.v[1] += ks;
+    sum.n[0] += cuts;
+    sum.n[1] += keeps;
+  };
+  int t0 = begin;
+  for (; t0 + (kUnroll - 1) * step < end; t0 += kUnroll * step) round(t0, Full{});
+  if (t0 < end) round(t0, Ragged{});
 }
 
 // Row sums (loss, k, cut, kept), weights and the result, by one block.
 __device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction,
                                               float* __restrict__ row_weight, float* __restrict__ loss,
                                               float* __restrict__ stats) {
-  __shared__ double total;
   const auto row_sum = [&](long long b, double (&row)[4]) {
     for (int i = 0; i < 4; ++i) row[i] = 0.;
     for (int s = 0; s < splits; ++s)
@@ -148,8 +191,7 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
     count[0] += reduction == MOLT_REDUCE_TOKEN ? row[3] : (row[3] > 0. ? 1. : 0.);
   }
   block_sum(count);
-  if (threadIdx.x == 0) total = count[0];
-  __syncthreads();
+  const double total = count[0];
   double sum[3] = {0., 0., 0.};
   for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
     if (b < blockDim.x) {
@@ -172,14 +214,18 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
   }
 }
 
-__global__ void __launch_bounds__(kThreads) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad, double* __restrict__ part) {
+template <bool REF, bool MASK>
+__global__ void __launch_bounds__(kThreads, 6) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad,
+                                                             double* __restrict__ part) {
   const long long b = blockIdx.x;
-  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
-  double sum[4] = {0., 0., 0., 0.};
-  policy_tokens(a, b, begin + threadIdx.x, end, kThreads, unit_grad, sum);
-  block_sum(sum);
-  if (threadIdx.x == 0)
-    for (int i = 0; i < 4; ++i) part[(b * a.splits + blockIdx.y) * 4 + i] = sum[i];
+  const int begin = blockIdx.y * a.part;
+  __shared__ double of_warp[4 * 32];
+  Sums<2, 2> sum;   // loss, k; cut, kept
+  policy_tokens<REF, MASK>(a, b, begin + threadIdx.x, min(a.seq, begin + a.part), kThreads, unit_grad, sum);
+  sum.join_warp();
+  if ((threadIdx.x & 31) == 0) sum.store(of_warp + (threadIdx.x >> 5), 32);
+  const double mine = join_block(of_warp, 4);
+  if (threadIdx.x < 4) part[(b * a.splits + blockIdx.y) * 4 + threadIdx.x] = mine;
 }
 
 __global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
@@ -189,6 +235,7 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __res
 }
 
 // The whole forward in one block: a warp takes one of the splits of a row.
+template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs a, int reduction, float* __restrict__ unit_grad,
                                                                      float* __restrict__ row_weight, float* __restrict__ loss,
                                                                      float* __restrict__ stats) {
@@ -196,26 +243,21 @@ __global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs 
   const int lane = threadIdx.x & 31, units = (int)a.batch * a.splits;
   for (int u = threadIdx.x >> 5; u < units; u += kOneBlock / 32) {
     const int b = u / a.splits, s = u - b * a.splits;
-    double sum[4] = {0., 0., 0., 0.};
-    policy_tokens(a, b, a.seq * s / a.splits + lane, a.seq * (s + 1) / a.splits, 32, unit_grad, sum);
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(~0u, sum[i], o);
-      if (lane == 0) part[u * 4 + i] = sum[i];
-    }
+    Sums<2, 2> sum;
+    policy_tokens<REF, MASK>(a, b, s * a.part + lane, min(a.seq, (s + 1) * a.part), 32, unit_grad, sum);
+    sum.join_warp();
+    if (lane == 0) sum.store(part + u * 4, 1);
   }
   __syncthreads();
   policy_finish(part, a.batch, a.splits, reduction, row_weight, loss, stats);
 }
 
-// Backward passes: a thread takes kUnroll tokens of one row, so that a block is one round of loads and stores.
-constexpr int kBackTokens = kThreads * kUnroll;
-
+// Backward passes: a block is one round of one row.
 __global__ void __launch_bounds__(kThreads) policy_backward_kernel(const float* __restrict__ unit_grad,
                                                                    const float* __restrict__ row_weight,
                                                                    const float* __restrict__ grad_loss,
                                                                    float* __restrict__ grad_logprob, long long seq) {
-  const long long b = blockIdx.x, first = b * seq, t0 = (long long)blockIdx.y * kBackTokens + threadIdx.x;
+  const long long b = blockIdx.x, first = b * seq, t0 = (long long)blockIdx.y * kRound + threadIdx.x;
   float u[kUnroll];
 #pragma unroll
   for (int j = 0; j < kUnroll; ++j) u[j] = t0 + j * kThreads < seq ? unit_grad[first + t0 + j * kThreads] : 0.f;
@@ -230,36 +272,37 @@ struct PreferenceArgs {
   const float *logprob, *ref;
   const uint8_t* mask;
   long long lp_stride, ref_stride, mask_stride;
-  long long pairs, seq;
-  int ref_per_token, splits, kind, average;
+  long long pairs;
+  int seq, ref_per_token, splits, part, kind, average;   // part: tokens of one of the splits of a row
   double beta, smoothing;
 };
 
-__device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long long i, long long begin, long long end, int step,
-                                                  double (&sum)[2]) {
-  int keeps = 0;
-  for (long long t0 = begin; t0 < end; t0 += kUnroll * step) {
-    float lp[kUnroll], ref[kUnroll];
+template <bool REF, bool MASK>
+__device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long long i, int begin, int end, int step,
+                                                  Sums<1, 1>& sum) {
+  const float* lp_row = a.logprob + i * a.lp_stride;
+  const float* ref_row = REF ? a.ref + i * a.ref_stride : nullptr;
+  const uint8_t* mask_row = MASK ? a.mask + i * a.mask_stride : nullptr;
+  const auto round = [&](int t0, auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    float d[kUnroll];
     bool kept[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long t = t0 + j * step;
-      kept[j] = t < end;
-      if (kept[j]) {
-        lp[j] = a.logprob[i * a.lp_stride + t];
-        ref[j] = a.ref != nullptr && a.ref_per_token ? a.ref[i * a.ref_stride + t] : 0.f;
-        kept[j] = a.mask == nullptr || a.mask[i * a.mask_stride + t] != 0;
-      }
+      const int t = FULL || t0 + j * step < end ? t0 + j * step : t0;   // a token of the row in any case
+      d[j] = REF ? lp_row[t] - ref_row[t] : lp_row[t];
+      kept[j] = (FULL || t0 + j * step < end) && (!MASK || mask_row[t] != 0);
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; j += 2) {
       // a pair of fp32 differences is added before it goes on in 64 bits: two roundings of the terms' magnitudes
-      const float d0 = kept[j] ? lp[j] - ref[j] : 0.f, d1 = kept[j + 1] ? lp[j + 1] - ref[j + 1] : 0.f;
-      sum[0] += d0 + d1;
-      keeps += (int)kept[j] + (int)kept[j + 1];
+      sum.v[0] += (kept[j] ? d[j] : 0.f) + (kept[j + 1] ? d[j + 1] : 0.f);
+      sum.n[0] += (int)kept[j] + (int)kept[j + 1];
     }
-  }
-  sum[1] += keeps;
+  };
+  int t0 = begin;
+  for (; t0 + (kUnroll - 1) * step < end; t0 += kUnroll * step) round(t0, Full{});
+  if (t0 < end) round(t0, Ragged{});
 }
 
 __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const double* part, float* __restrict__ seq_grad,
@@ -306,16 +349,17 @@ __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const
   if (threadIdx.x == 0) loss_out[0] = (float)total[0];
 }
 
-__global__ void __launch_bounds__(kThreads) preference_kernel(PreferenceArgs a, double* __restrict__ part) {
+template <bool REF, bool MASK>
+__global__ void __launch_bounds__(kThreads, 8) preference_kernel(PreferenceArgs a, double* __restrict__ part) {
   const long long i = blockIdx.x;
-  const long long begin = a.seq * blockIdx.y / a.splits, end = a.seq * (blockIdx.y + 1) / a.splits;
-  double sum[2] = {0., 0.};
-  preference_tokens(a, i, begin + threadIdx.x, end, kThreads, sum);
-  block_sum(sum);
-  if (threadIdx.x == 0) {
-    part[(i * a.splits + blockIdx.y) * 2] = sum[0];
-    part[(i * a.splits + blockIdx.y) * 2 + 1] = sum[1];
-  }
+  const int begin = blockIdx.y * a.part;
+  __shared__ double of_warp[2 * 32];
+  Sums<1, 1> sum;   // difference to the reference; kept
+  preference_tokens<REF, MASK>(a, i, begin + threadIdx.x, min(a.seq, begin + a.part), kThreads, sum);
+  sum.join_warp();
+  if ((threadIdx.x & 31) == 0) sum.store(of_warp + (threadIdx.x >> 5), 32);
+  const double mine = join_block(of_warp, 2);
+  if (threadIdx.x < 2) part[(i * a.splits + blockIdx.y) * 2 + threadIdx.x] = mine;
 }
 
 __global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
@@ -324,19 +368,17 @@ __global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs 
   preference_finish(a, part, seq_grad, rewards, loss);
 }
 
+template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kOneBlock) preference_one_block_kernel(PreferenceArgs a, float* __restrict__ seq_grad,
                                                                          float* __restrict__ rewards, float* __restrict__ loss) {
   __shared__ double part[kOneBlockRows * 2];
   const int lane = threadIdx.x & 31, units = (int)(2 * a.pairs) * a.splits;
   for (int u = threadIdx.x >> 5; u < units; u += kOneBlock / 32) {
     const int i = u / a.splits, s = u - i * a.splits;
-    double sum[2] = {0., 0.};
-    preference_tokens(a, i, a.seq * s / a.splits + lane, a.seq * (s + 1) / a.splits, 32, sum);
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(~0u, sum[k], o);
-      if (lane == 0) part[u * 2 + k] = sum[k];
-    }
+    Sums<1, 1> sum;
+    preference_tokens<REF, MASK>(a, i, s * a.part + lane, min(a.seq, (s + 1) * a.part), 32, sum);
+    sum.join_warp();
+    if (lane == 0) sum.store(part + u * 2, 1);
   }
   __syncthreads();
   preference_finish(a, part, seq_grad, rewards, loss);
@@ -346,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) preference_backward_kernel(const uin
                                                                        const float* __restrict__ seq_grad,
                                                                        const float* __restrict__ grad_loss,
                                                                        float* __restrict__ grad_logprob, long long seq) {
-  const long long i = blockIdx.x, t0 = (long long)blockIdx.y * kBackTokens + threadIdx.x;
+  const long long i = blockIdx.x, t0 = (long long)blockIdx.y * kRound + threadIdx.x;
   bool kept[kUnroll];
 #pragma unroll
   for (int j = 0; j < kUnroll; ++j)
@@ -404,18 +446,24 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
   a.logprob = logprob; a.old = old_logprob; a.ref = ref_logprob; a.advantage = advantage; a.mask = mask;
   a.lp_stride = row_strides[0]; a.old_stride = row_strides[1]; a.ref_stride = row_strides[2]; a.adv_stride = row_strides[3];
   a.mask_stride = row_strides[4];
-  a.batch = batch; a.seq = seq; a.per_token = advantage_per_token != 0; a.splits = splits_for(batch, seq);
+  a.batch = batch; a.seq = (int)seq; a.per_token = advantage_per_token != 0;
+  a.splits = splits_for(batch, seq); a.part = part_tokens(batch, seq);
   a.log_high = log1p(clip_high); a.log_low = log1p(-clip_low);
   a.log_high_f = (float)a.log_high; a.log_low_f = (float)a.log_low;
   a.high = (float)(1. + clip_high); a.low = (float)(1. - clip_low); a.kl_coef = (float)kl_coef;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (needed == 0) {
     a.splits = one_block_splits(batch);
-    policy_one_block_kernel<<<1, kOneBlock, 0, s>>>(a, reduction, unit_grad, row_weight, loss, stats);
+    a.part = ((int)seq + a.splits - 1) / a.splits;
+    const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_one_block_kernel<true, true> : policy_one_block_kernel<true, false>)
+                                               : (mask != nullptr ? policy_one_block_kernel<false, true> : policy_one_block_kernel<false, false>);
+    kernel<<<1, kOneBlock, 0, s>>>(a, reduction, unit_grad, row_weight, loss, stats);
     return launch_status("policy_one_block_kernel");
   }
   auto* part = reinterpret_cast<double*>(workspace);
-  policy_kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
+  const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_kernel<true, true> : policy_kernel<true, false>)
+                                             : (mask != nullptr ? policy_kernel<false, true> : policy_kernel<false, false>);
+  kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
   if (int rc = launch_status("policy_kernel")) return rc;
   policy_finish_kernel<<<1, 1024, 0, s>>>(part, batch, a.splits, reduction, row_weight, loss, stats);
   return launch_status("policy_finish_kernel");
@@ -427,7 +475,7 @@ extern "C" int molt_policy_loss_bwd(const float* unit_grad, const float* row_wei
   if (int rc = check_sizes(who, batch, seq)) return rc;
   if (batch == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(unit_grad && row_weight && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
-  const dim3 grid((unsigned)batch, (unsigned)((seq + kBackTokens - 1) / kBackTokens));
+  const dim3 grid((unsigned)batch, (unsigned)((seq + kRound - 1) / kRound));
   policy_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(unit_grad, row_weight, grad_loss, grad_logprob,
                                                                                        seq);
   return launch_status("policy_backward_kernel");
@@ -459,16 +507,23 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
   PreferenceArgs a;
   a.logprob = logprob; a.ref = ref_logprob; a.mask = mask;
   a.lp_stride = row_strides[0]; a.ref_stride = row_strides[1]; a.mask_stride = row_strides[2];
-  a.pairs = pairs; a.seq = seq; a.ref_per_token = ref_per_token != 0; a.splits = splits_for(2 * pairs, seq);
+  a.pairs = pairs; a.seq = (int)seq; a.ref_per_token = ref_per_token != 0;
+  a.splits = splits_for(2 * pairs, seq); a.part = part_tokens(2 * pairs, seq);
+  const bool tokens = ref_logprob != nullptr && ref_per_token;   // the reference is subtracted token by token
   a.kind = kind; a.average = average != 0; a.beta = beta; a.smoothing = smoothing;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (needed == 0) {
     a.splits = one_block_splits(2 * pairs);
-    preference_one_block_kernel<<<1, kOneBlock, 0, s>>>(a, seq_grad, rewards, loss);
+    a.part = ((int)seq + a.splits - 1) / a.splits;
+    const auto kernel = tokens ? (mask != nullptr ? preference_one_block_kernel<true, true> : preference_one_block_kernel<true, false>)
+                               : (mask != nullptr ? preference_one_block_kernel<false, true> : preference_one_block_kernel<false, false>);
+    kernel<<<1, kOneBlock, 0, s>>>(a, seq_grad, rewards, loss);
     return launch_status("preference_one_block_kernel");
   }
   auto* part = reinterpret_cast<double*>(workspace);
-  preference_kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
+  const auto kernel = tokens ? (mask != nullptr ? preference_kernel<true, true> : preference_kernel<true, false>)
+                             : (mask != nullptr ? preference_kernel<false, true> : preference_kernel<false, false>);
+  kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
   if (int rc = launch_status("preference_kernel")) return rc;
   preference_finish_kernel<<<1, 1024, 0, s>>>(a, part, seq_grad, rewards, loss);
   return launch_status("preference_finish_kernel");
@@ -482,7 +537,7 @@ extern "C" int molt_preference_loss_bwd(const uint8_t* mask, int64_t mask_stride
   if (pairs == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(seq_grad && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   if (int rc = check_stride(who, "mask", mask_stride, seq)) return rc;
-  const dim3 grid((unsigned)(2 * pairs), (unsigned)((seq + kBackTokens - 1) / kBackTokens));
+  const dim3 grid((unsigned)(2 * pairs), (unsigned)((seq + kRound - 1) / kRound));
   preference_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(mask, mask_stride, seq_grad, grad_loss,
                                                                                            grad_logprob, seq);
   return launch_status("preference_backward_kernel");
