@@ -11,7 +11,7 @@
 namespace molt {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kFinish = 512;
 
 // Sums of one thread: N in 64 bits, and M counts.
 template <int N, int M>
@@ -37,12 +37,17 @@ struct Sums {
   }
 };
 
-// Adds up, over a block and in a fixed order, what `store` left of every warp in part[value][warp]; thread i returns value i.
+// Adds up, over a block and in a fixed order, what `store` left of every warp in part[value][warp]: warp i does value i, and
+// its lane 0 returns it.
 __device__ __forceinline__ double join_block(const double* part, int values) {
   __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.;
-  if (threadIdx.x < values)
-    for (int w = 0; w < (blockDim.x >> 5); ++w) sum += part[threadIdx.x * 32 + w];
+  if (warp < values) {
+    sum = lane < (blockDim.x >> 5) ? part[warp * 32 + lane] : 0.;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  }
   return sum;
 }
 
@@ -50,16 +55,17 @@ __device__ __forceinline__ double join_block(const double* part, int values) {
 template <int N>
 __device__ __forceinline__ void block_sum(double (&v)[N]) {
   __shared__ double part[N * 32], total[N];
-  Sums<N, 1> sums;
-  for (int i = 0; i < N; ++i) sums.v[i] = v[i];
-  sums.join_warp();
-  if ((threadIdx.x & 31) == 0)
-    for (int i = 0; i < N; ++i) part[i * 32 + (threadIdx.x >> 5)] = sums.v[i];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
+    if (lane == 0) part[i * 32 + warp] = v[i];
+  }
   const double mine = join_block(part, N);
-  if (threadIdx.x < N) total[threadIdx.x] = mine;
+  if (lane == 0 && warp < N) total[warp] = mine;
   __syncthreads();
   for (int i = 0; i < N; ++i) v[i] = total[i];
-  __syncthreads();
 }
 
 using Full = std::integral_constant<bool, true>;
@@ -178,6 +184,7 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
                                               float* __restrict__ stats) {
   const auto row_sum = [&](long long b, double (&row)[4]) {
     for (int i = 0; i < 4; ++i) row[i] = 0.;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s)
       for (int i = 0; i < 4; ++i) row[i] += part[(b * splits + s) * 4 + i];
   };
@@ -225,10 +232,11 @@ __global__ void __launch_bounds__(kThreads, 6) policy_kernel(PolicyArgs a, float
   sum.join_warp();
   if ((threadIdx.x & 31) == 0) sum.store(of_warp + (threadIdx.x >> 5), 32);
   const double mine = join_block(of_warp, 4);
-  if (threadIdx.x < 4) part[(b * a.splits + blockIdx.y) * 4 + threadIdx.x] = mine;
+  const int value = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0 && value < 4) part[(b * a.splits + blockIdx.y) * 4 + value] = mine;
 }
 
-__global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
+__global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
                                                              int reduction, float* __restrict__ row_weight,
                                                              float* __restrict__ loss, float* __restrict__ stats) {
   policy_finish(part, batch, splits, reduction, row_weight, loss, stats);
@@ -313,6 +321,7 @@ __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const
     for (int side = 0; side < 2; ++side) {
       const long long i = p + side * a.pairs;
       double sum = 0., kept = 0.;
+#pragma unroll 4
       for (int k = 0; k < a.splits; ++k) {
         sum += part[(i * a.splits + k) * 2];
         kept += part[(i * a.splits + k) * 2 + 1];
@@ -359,10 +368,11 @@ __global__ void __launch_bounds__(kThreads, 8) preference_kernel(PreferenceArgs 
   sum.join_warp();
   if ((threadIdx.x & 31) == 0) sum.store(of_warp + (threadIdx.x >> 5), 32);
   const double mine = join_block(of_warp, 2);
-  if (threadIdx.x < 2) part[(i * a.splits + blockIdx.y) * 2 + threadIdx.x] = mine;
+  const int value = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0 && value < 2) part[(i * a.splits + blockIdx.y) * 2 + value] = mine;
 }
 
-__global__ void __launch_bounds__(1024) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
+__global__ void __launch_bounds__(kFinish) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
                                                                  float* __restrict__ seq_grad, float* __restrict__ rewards,
                                                                  float* __restrict__ loss) {
   preference_finish(a, part, seq_grad, rewards, loss);
@@ -465,7 +475,7 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
                                              : (mask != nullptr ? policy_kernel<false, true> : policy_kernel<false, false>);
   kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
   if (int rc = launch_status("policy_kernel")) return rc;
-  policy_finish_kernel<<<1, 1024, 0, s>>>(part, batch, a.splits, reduction, row_weight, loss, stats);
+  policy_finish_kernel<<<1, kFinish, 0, s>>>(part, batch, a.splits, reduction, row_weight, loss, stats);
   return launch_status("policy_finish_kernel");
 }
 
@@ -525,7 +535,7 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
                              : (mask != nullptr ? preference_kernel<false, true> : preference_kernel<false, false>);
   kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
   if (int rc = launch_status("preference_kernel")) return rc;
-  preference_finish_kernel<<<1, 1024, 0, s>>>(a, part, seq_grad, rewards, loss);
+  preference_finish_kernel<<<1, kFinish, 0, s>>>(a, part, seq_grad, rewards, loss);
   return launch_status("preference_finish_kernel");
 }
 
