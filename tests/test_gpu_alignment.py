@@ -185,6 +185,92 @@ def test_token_logprobs_shapes_strides_and_offsets(native_library):
     assert torch.equal(a, b) and torch.equal(g, h)
 
 
+def _check_all_forms(logits, ids, temperature, out=None):
+    from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
+
+    weight = torch.linspace(-2.0, 2.0, len(ids), device="cuda")
+    want, probs, kept, bound = _exact_logprobs(logits, ids, temperature)
+    want_grad = _exact_grad(probs, ids, kept, weight, temperature)
+    leaf = logits.detach().requires_grad_()
+    lp = token_logprobs(leaf, ids, temperature)
+    _close(lp.detach(), want, bound)
+    _check_grad(torch.autograd.grad(lp, leaf, weight)[0], want_grad, bound, weight, temperature, logits.dtype)
+    lp, grad = token_logprobs_with_grad(logits, ids, weight, temperature, out=out)
+    _close(lp, want, bound)
+    _check_grad(grad, want_grad, bound, weight, temperature, logits.dtype)
+
+
+# Vectors of 16 bytes around the borders of the batches (512 vectors per block) and of the ring (5 batches), and of the
+# small blocks (512 vectors); the elements behind them; 3 rows are spread over many blocks, 700 are not.
+BORDERS = [1, 63, 64, 511, 512, 513, 1023, 1024, 1025, 2559, 2560, 2561, 3073, 3136, 5119, 5120, 5121, 5632, 8192]
+
+
+@pytest.mark.parametrize("vectors", BORDERS)
+@pytest.mark.parametrize("rows,dtype", [(3, torch.bfloat16), (3, torch.float32), (700, torch.bfloat16)])
+def test_token_logprobs_at_the_borders_of_their_blocks(native_library, vectors, rows, dtype):
+    gen = _gen(vectors)
+    per = 16 // dtype.itemsize
+    for extra in (0, per - 1):
+        vocab = vectors * per + extra
+        logits = (torch.randn(rows, vocab, device="cuda", generator=gen) * 2).to(dtype)
+        ids = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+        ids[0], ids[1] = vocab - 1, 0
+        _check_all_forms(logits, ids, 0.9)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(2, 700_001, torch.bfloat16), (2, 1_300_000, torch.float32), (70_000, 5, torch.float32),
+                                              (66_000, 131, torch.bfloat16)])
+def test_token_logprobs_of_long_rows_and_many_rows(native_library, rows, vocab, dtype):
+    gen = _gen(rows)
+    logits = torch.empty(rows, vocab, dtype=dtype, device="cuda").normal_(0.0, 3.0, generator=gen)
+    ids = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+    ids[-1] = -1
+    _check_all_forms(logits, ids, 1.0)
+
+
+def test_token_logprobs_with_every_id_ignored_and_in_inference_mode(native_library):
+    from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
+
+    logits = torch.full((5, 9000), float("nan"), device="cuda", requires_grad=True)
+    ids = torch.full((5,), -100, device="cuda")
+    lp = token_logprobs(logits, ids)
+    lp.sum().backward()
+    assert not bool(lp.any()) and not bool(logits.grad.any())
+    with torch.inference_mode():
+        x = torch.zeros(5, 9000, device="cuda")
+        lp, grad = token_logprobs_with_grad(x, ids + 101, out=x)
+        _close(lp, torch.full((5,), -math.log(9000), device="cuda", dtype=torch.float64), torch.full((5,), 200 * U, device="cuda"))
+        assert grad is x and float(grad[0, 1]) == pytest.approx(1 - 1 / 9000, rel=1e-6)
+        _close(token_logprobs(torch.zeros(5, 9000, device="cuda"), ids + 101), lp.double(), torch.full((5,), 400 * U, device="cuda"))
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 151936), (40, 40000)])
+def test_token_logprobs_replayed_as_graphs(native_library, rows, vocab):
+    """Rows spread over clusters of blocks, recorded once and replayed on other logits and ids, ignored ones among them."""
+    from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
+
+    gen = _gen(rows)
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    out = torch.empty_like(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        token_logprobs(x, ids), token_logprobs_with_grad(x, ids, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        scored = token_logprobs(x, ids)
+        lp, _ = token_logprobs_with_grad(x, ids, out=out)
+    for step in range(3):
+        x.normal_(0.0, 2.0, generator=gen)
+        ids.random_(0, vocab, generator=gen)
+        ids[step] = -100
+        graph.replay()
+        want = token_logprobs_with_grad(x, ids)
+        assert torch.equal(lp, want[0]) and torch.equal(out, want[1]) and torch.equal(scored, token_logprobs(x, ids))
+
+
 def test_token_logprobs_refusals(native_library):
     from molt_b200.core.errors import CapabilityError
     from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
