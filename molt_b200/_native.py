@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import threading
 from array import array
+from contextlib import nullcontext
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -239,6 +240,14 @@ def stream_handle(device: Optional[torch.device] = None) -> int:
         device = torch.device(device)
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)   # no Stream object: this stands in front of every call
+
+
+_HERE = nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one; costs next to nothing where it is already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(tensor: Optional[torch.Tensor]) -> Optional[int]:

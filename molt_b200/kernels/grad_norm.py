@@ -54,7 +54,7 @@ def _launch(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, 
     lib = _native.library()
     scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(count), device)
     result = torch.empty(2, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
+    with _native.on_device(device):
         if outs is None:
             _native.check(lib.molt_grad_norm(items.buffer_info()[0], count, kind, 1.0, max_norm, result.data_ptr(),
                                              scratch.data_ptr(), scratch.numel(), _native.stream_handle(device)))

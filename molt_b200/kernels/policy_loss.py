@@ -83,7 +83,7 @@ def _policy_forward(call, trained: bool):
     nbytes = lib.molt_policy_loss_workspace_bytes(batch, seq)
     scratch = _native.workspace(nbytes, device) if nbytes else None
     strides = (ctypes.c_int64 * 5)(*map(_row_stride, (lp, old, ref, advantages, mask)))
-    with torch.cuda.device(device):
+    with _native.on_device(device):
         _native.check(lib.molt_policy_loss_fwd(
             lp.data_ptr(), old.data_ptr(), _native.ptr(ref), advantages.data_ptr(), int(advantages.dim() == 2),
             _native.ptr(mask), strides, batch, seq, clip_low, clip_high, kl_coef, reduction, unit, weight, loss.data_ptr(),
@@ -109,7 +109,7 @@ class _PolicyLossFunction(torch.autograd.Function):
         batch, seq = ctx.shape
         grad = kept.new_empty((batch, seq))
         unit = kept.data_ptr()
-        with torch.cuda.device(kept.device):
+        with _native.on_device(kept.device):
             _native.check(_native.library().molt_policy_loss_bwd(unit, unit + 4 * batch * seq, grad_loss.data_ptr(), grad.data_ptr(),
                                                                  batch, seq, _native.stream_handle(kept.device)))
         return grad, None, None
@@ -144,7 +144,7 @@ def clipped_policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
         stats = told[0]
     else:
         loss, stats, _ = _policy_forward((logprobs, *call), False)
-    return PolicyLoss(loss, *stats.unbind())
+    return PolicyLoss(loss, stats[0], stats[1])
 
 
 def _preference_forward(call, trained: bool):
@@ -160,7 +160,7 @@ def _preference_forward(call, trained: bool):
     nbytes = lib.molt_preference_loss_workspace_bytes(pairs, seq)
     scratch = _native.workspace(nbytes, device) if nbytes else None
     strides = (ctypes.c_int64 * 3)(*map(_row_stride, (lp, ref, mask)))
-    with torch.cuda.device(device):
+    with _native.on_device(device):
         _native.check(lib.molt_preference_loss_fwd(
             lp.data_ptr(), _native.ptr(ref), int(ref is not None and ref.dim() == 2), _native.ptr(mask), strides, pairs, seq,
             beta, smoothing, kind, average, _native.ptr(seq_grad), rewards.data_ptr(), loss.data_ptr(), _native.ptr(scratch), nbytes,
@@ -185,7 +185,7 @@ class _PreferenceLossFunction(torch.autograd.Function):
         mask, seq_grad = ctx.saved_tensors
         sequences, seq = ctx.shape
         grad = seq_grad.new_empty((sequences, seq))
-        with torch.cuda.device(grad.device):
+        with _native.on_device(grad.device):
             _native.check(_native.library().molt_preference_loss_bwd(
                 _native.ptr(mask), _row_stride(mask), seq_grad.data_ptr(), grad_loss.data_ptr(), grad.data_ptr(), sequences // 2, seq,
                 _native.stream_handle(grad.device)))
@@ -220,4 +220,4 @@ def preference_loss(logprobs: torch.Tensor, ref_logprobs: Optional[torch.Tensor]
         rewards = told[0]
     else:
         loss, rewards, _, _ = _preference_forward((logprobs, *call), False)
-    return PreferenceLoss(loss, *rewards.unbind())
+    return PreferenceLoss(loss, rewards[0], rewards[1])

@@ -27,6 +27,8 @@ def _check(logits: torch.Tensor, token_ids: torch.Tensor) -> int:
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """``[rows, vocab]`` with neighbouring columns: a view where the strides allow it, else a copy."""
+    if logits.dim() == 2 and logits.is_contiguous():
+        return logits
     rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if (rows.shape[1] != 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and 0 < rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()
@@ -40,7 +42,7 @@ def _stride(rows: torch.Tensor) -> int:
 def _forward(rows: torch.Tensor, ids: torch.Tensor, temperature: float, stats: Optional[torch.Tensor]) -> torch.Tensor:
     device = rows.device
     logprobs = torch.empty(ids.shape, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
+    with _native.on_device(device):
         _native.check(_native.library().molt_token_logprob_fwd(
             rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), temperature, logprobs.data_ptr(),
             _native.ptr(stats), rows.shape[0], rows.shape[1], _native.stream_handle(device)))
@@ -64,7 +66,7 @@ class _TokenLogprobs(torch.autograd.Function):
         rows, ids, stats = ctx.saved_tensors
         grad_output = grad_output.contiguous()
         grad = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
-        with torch.cuda.device(rows.device):
+        with _native.on_device(rows.device):
             _native.check(_native.library().molt_token_logprob_bwd(
                 rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), stats.data_ptr(), grad_output.data_ptr(),
                 ctx.temperature, grad.data_ptr(), grad.shape[1], rows.shape[0], rows.shape[1],
@@ -84,7 +86,6 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, temperature: f
     return _forward(_rows(logits), token_ids.contiguous(), float(temperature), None)
 
 
-@torch.no_grad()
 def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weight: Optional[torch.Tensor] = None,
                              temperature: float = 1.0, out: Optional[torch.Tensor] = None
                              ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -95,25 +96,27 @@ def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weig
     be ``logits`` itself, which it then overwrites (it must not overlap them in any other way).  Nothing is recorded for
     autograd."""
     dtype = _check(logits, token_ids)
-    rows, ids = _rows(logits), token_ids.contiguous()
+    rows, ids = _rows(logits.detach()), token_ids.contiguous()
     if weight is not None:
         if weight.shape != token_ids.shape or weight.dtype != torch.float32 or weight.device != logits.device:
             raise ValueError("weight must be float32 of the shape of token_ids on the logits' device")
-        weight = weight.contiguous()
+        weight = weight.detach().contiguous()
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out must have the logits' shape, dtype and device")
     elif out.requires_grad:
         raise ValueError("out must not require a gradient")
-    try:
-        target = out.view(-1, out.shape[-1])
-    except RuntimeError as exc:
-        raise ValueError("out must be a tensor of rows with one stride") from exc
+    target = out
+    if out.dim() != 2:
+        try:
+            target = out.view(-1, out.shape[-1])
+        except RuntimeError as exc:
+            raise ValueError("out must be a tensor of rows with one stride") from exc
     if target.shape[1] != 1 and target.stride(1) != 1:
         raise ValueError("out must have neighbouring columns")
     logprobs = torch.empty(token_ids.shape, dtype=torch.float32, device=logits.device)
-    with torch.cuda.device(logits.device):
+    with _native.on_device(logits.device):
         _native.check(_native.library().molt_token_logprob_grad(
             rows.data_ptr(), dtype, _stride(rows), ids.data_ptr(), _native.ptr(weight), float(temperature), logprobs.data_ptr(),
             target.data_ptr(), _stride(target), rows.shape[0], rows.shape[1], _native.stream_handle(logits.device)))
