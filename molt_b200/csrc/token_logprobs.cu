@@ -562,45 +562,56 @@ int launch_clusters(const char* what, void (*kernel)(Params...), int64_t rows, i
   return launch_status(what);
 }
 
-// Rows of at most 512 vectors (4096 bf16, 2048 fp32) take small blocks, many to an SM; longer ones large blocks, and a
-// cluster of them (a power of two, at most 8) where one block would not do:
+// Threads for a row of `vectors` 16-byte vectors.  A block that is done too soon spends its time on being launched, on its
+// first loads and on its join: it is made as small as leaves a thread 13 vectors (16384 rows x 8192 bf16, forward: 99 us with
+// 512 threads, SMALL with 64), but not so small that there are too few threads for the device (while a thread keeps 4).
+int threads_for(int64_t rows, int64_t vectors, int most, int resident) {
+  int threads = 64;
+  while (threads < most && vectors >= 2 * threads * 13) threads *= 2;
+  while (threads < most && rows * threads < (int64_t)148 * resident && vectors >= 2 * threads * 4) threads *= 2;
+  return threads;
+}
+
+// Where the largest block would not do, a cluster of them takes a row (a power of two, at most 8):
 // * with gradient, until a thread has at most 20 vectors, so that the rows in flight stay in the L2;
 // * in both directions, as long as the rows alone do not fill the device and a thread keeps at least 4 vectors.
 template <typename T>
 int launch_forward(const void* logits, int64_t row_stride, const int64_t* ids, float temperature, float* logprob, float* stats,
                    int64_t rows, int64_t vocab, cudaStream_t s) {
+  constexpr int kResident = sizeof(T) == 2 ? 2048 : 1536;   // threads per SM: 32 registers each, or 40
   const int64_t vectors = vocab / Vec<T>::kElements;
-  auto* x = reinterpret_cast<const T*>(logits);
-  auto* id = reinterpret_cast<const long long*>(ids);
-  auto* st = reinterpret_cast<float2*>(stats);
-  if (vectors <= 64 * 8)
-    return launch_clusters("token_logprob row_kernel", row_kernel<T, 64, 2, 16>, rows, 1, 64, 0, s, x, row_stride, id, 1.f / temperature,
-                           logprob, st, vocab);
+  const int threads = threads_for(rows, vectors, 512, kResident);
+  const auto launch = [&](auto kernel, int cluster) {
+    return launch_clusters("token_logprob row_kernel", kernel, rows, cluster, threads, 0, s, reinterpret_cast<const T*>(logits), row_stride,
+                           reinterpret_cast<const long long*>(ids), 1.f / temperature, logprob, reinterpret_cast<float2*>(stats), vocab);
+  };
+  if (threads == 64) return launch(row_kernel<T, 64, 4, kResident / 64>, 1);
+  if (threads == 128) return launch(row_kernel<T, 128, 4, kResident / 128>, 1);
+  if (threads == 256) return launch(row_kernel<T, 256, 4, kResident / 256>, 1);
   int cluster = 1;
   while (cluster < 8 && rows * cluster < 148 * 2 && vectors >= cluster * 512 * 4) cluster *= 2;
-  return launch_clusters("token_logprob row_kernel", row_kernel<T, 512, 4, sizeof(T) == 2 ? 4 : 3>, rows, cluster, 512, 0, s, x, row_stride,
-                         id, 1.f / temperature, logprob, st, vocab);
+  return launch(row_kernel<T, 512, 4, kResident / 512>, cluster);
 }
 
 template <typename T>
 int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, const float* weight, float temperature, float* logprob,
                 void* grad, int64_t grad_stride, int64_t rows, int64_t vocab, cudaStream_t s) {
-  constexpr size_t kSlots = kRing * kRingBatch * sizeof(uint4);
+  constexpr int kResident = 1280;   // threads per SM: 48 registers and 160 bytes of the ring each
   const int64_t vectors = vocab / Vec<T>::kElements;
-  auto* x = reinterpret_cast<const T*>(logits);
-  auto* id = reinterpret_cast<const long long*>(ids);
-  auto* g = reinterpret_cast<T*>(grad);
-  const auto launch = [&](auto kernel, int cluster, int threads) {
-    return launch_clusters("token_logprob row_grad_kernel", kernel, rows, cluster, threads, threads * kSlots, s, x, row_stride, id, weight,
-                           1.f / temperature, logprob, g, grad_stride, vocab);
+  const int threads = threads_for(rows, vectors, 256, kResident);
+  const auto launch = [&](auto kernel, int cluster) {
+    return launch_clusters("token_logprob row_grad_kernel", kernel, rows, cluster, threads, threads * kRing * kRingBatch * sizeof(uint4), s,
+                           reinterpret_cast<const T*>(logits), row_stride, reinterpret_cast<const long long*>(ids), weight,
+                           1.f / temperature, logprob, reinterpret_cast<T*>(grad), grad_stride, vocab);
   };
-  if (vectors <= 64 * 8) return launch(row_grad_kernel<T, 64, 1, 16>, 1, 64);
+  if (threads == 64) return launch(row_grad_kernel<T, 64, 1, kResident / 64>, 1);
+  if (threads == 128) return launch(row_grad_kernel<T, 128, 1, kResident / 128>, 1);
   int cluster = 1;
   while (cluster < 8 && (vectors > cluster * 256 * 20 || (rows * cluster < 148 * 4 && vectors >= cluster * 256 * 4))) cluster *= 2;
-  if (cluster == 1) return launch(row_grad_kernel<T, 256, 1, 5>, 1, 256);
-  if (cluster == 2) return launch(row_grad_kernel<T, 256, 2, 5>, 2, 256);
-  if (cluster == 4) return launch(row_grad_kernel<T, 256, 4, 5>, 4, 256);
-  return launch(row_grad_kernel<T, 256, 8, 5>, 8, 256);
+  if (cluster == 1) return launch(row_grad_kernel<T, 256, 1, kResident / 256>, 1);
+  if (cluster == 2) return launch(row_grad_kernel<T, 256, 2, kResident / 256>, 2);
+  if (cluster == 4) return launch(row_grad_kernel<T, 256, 4, kResident / 256>, 4);
+  return launch(row_grad_kernel<T, 256, 8, kResident / 256>, 8);
 }
 
 }  // namespace
