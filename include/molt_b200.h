@@ -350,14 +350,14 @@ int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, c
  * they hold.  ref_logprob may be NULL (k = 0).  advantage is [batch, seq] or, with advantage_per_token == 0, [batch].
  * row_strides: elements between the rows of logprob, old, ref, advantage (between its entries when it is [batch]), mask.
  * loss[0]; stats[2] = mean k, mean of 1[the clamp cut the gradient].  For the backward (unit_grad NULL: not wanted):
- * unit_grad [batch, seq] receives d l / d logprob per token, zero behind the mask, and row_weight [batch] the weight of
- * a kept token of the row.  A small batch needs no workspace (0 bytes, NULL).  The clamp's border is decided in 64 bits, sums are kept in 64 bits, in a fixed order. */
+ * unit_grad [batch, seq] receives d l / d logprob per token, zero behind the mask, and row_weight [batch + 1] the
+ * weights that a kept token's share of the mean is the product of: its row's, and behind them one for all.  A small batch needs no workspace (0 bytes, NULL).  The clamp's border is decided in 64 bits, sums are kept in 64 bits, in a fixed order. */
 size_t molt_policy_loss_workspace_bytes(int64_t batch, int64_t seq);
 int molt_policy_loss_fwd(const float* logprob, const float* old_logprob, const float* ref_logprob, const float* advantage,
                          int advantage_per_token, const uint8_t* mask, const int64_t row_strides[5], int64_t batch,
                          int64_t seq, double clip_low, double clip_high, double kl_coef, int reduction, float* unit_grad,
                          float* row_weight, float* loss, float* stats, void* workspace, size_t workspace_bytes, uintptr_t stream);
-/* grad_logprob[b, t] = grad_loss[0] * row_weight[b] * unit_grad[b, t] (exactly zero where unit_grad is). */
+/* grad_logprob[b, t] = grad_loss[0] * row_weight[batch] * row_weight[b] * unit_grad[b, t] (exactly zero where unit_grad is). */
 int molt_policy_loss_bwd(const float* unit_grad, const float* row_weight, const float* grad_loss, float* grad_logprob,
                          int64_t batch, int64_t seq, uintptr_t stream);
 

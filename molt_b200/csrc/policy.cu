@@ -19,7 +19,7 @@ struct Sums {
   double v[N] = {};
   int n[M] = {};
 
-  // Sums of the warp, in lane 0.
+  // Sums of the warp, in all its lanes.
   __device__ __forceinline__ void join_warp() {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -28,7 +28,7 @@ struct Sums {
 #pragma unroll
     for (int i = 0; i < M; ++i) n[i] = __reduce_add_sync(~0u, n[i]);
   }
-  // Lane 0's sums as N + M doubles.
+  // The sums as N + M doubles.
   __device__ __forceinline__ void store(double* to, int stride) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) to[i * stride] = v[i];
@@ -91,6 +91,35 @@ constexpr int kOneBlock = 1024, kOneBlockRows = 256, kOneBlockTokens = 8192;
 bool one_block(int64_t rows, int64_t seq) { return rows <= kOneBlockRows && rows * seq <= kOneBlockTokens; }
 // Warps of the one block that share a row.
 int one_block_splits(int64_t rows) { return rows >= kOneBlock / 32 ? 1 : (int)(kOneBlock / 32 / rows); }
+
+// Many short rows: a warp takes a row, a block eight at a time (16384 x 128 tokens with a block per row: 85 us).
+constexpr int kWarpRows = 2048, kWarpTokens = kRound, kWarps = kThreads / 32;
+bool warp_rows(int64_t rows, int64_t seq) { return rows >= kWarpRows && seq <= kWarpTokens; }
+int warp_row_blocks(int64_t rows) { return (int)((rows + kWarps - 1) / kWarps < 148 * 8 ? (rows + kWarps - 1) / kWarps : 148 * 8); }
+
+// Sums over the splits of row b of its N values.  A row of many splits is added up by a warp, whose lanes all call this.
+constexpr int kSplitsPerThread = 8;
+template <int N>
+__device__ __forceinline__ void row_sums(const double* part, long long b, int splits, double (&row)[N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < N; ++i) row[i] = 0.;
+  if (splits <= kSplitsPerThread) {
+    for (int s = 0; s < splits; ++s)
+      for (int i = 0; i < N; ++i) row[i] += part[(b * splits + s) * N + i];
+    return;
+  }
+  for (int s = lane; s < splits; s += 32)
+    for (int i = 0; i < N; ++i) row[i] += part[(b * splits + s) * N + i];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) row[i] += __shfl_xor_sync(~0u, row[i], o);
+}
+// The rows this thread works on in a finishing block: each thread its own, or each warp its own.
+__device__ __forceinline__ long long first_row(int splits) { return splits <= kSplitsPerThread ? threadIdx.x : threadIdx.x >> 5; }
+__device__ __forceinline__ int row_step(int splits) { return splits <= kSplitsPerThread ? blockDim.x : blockDim.x >> 5; }
+__device__ __forceinline__ bool speaks(int splits) { return splits <= kSplitsPerThread || (threadIdx.x & 31) == 0; }
 
 // ---- clipped policy loss -------------------------------------------------------------------------------------------
 struct PolicyArgs {
@@ -158,8 +187,10 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
       float g = cut || adv[j] == 0.f ? 0.f : -r * adv[j];
       if (REF) {
         const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
-        l += a.kl_coef * k;
-        g -= a.kl_coef * (k + e);   // exp(e) - 1
+        if (a.kl_coef != 0.f) {
+          l += a.kl_coef * k;
+          g -= a.kl_coef * (k + e);   // exp(e) - 1
+        }
         ks += kept[j] ? k : 0.f;
       }
       loss += kept[j] ? l : 0.f;
@@ -178,51 +209,46 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
   if (t0 < end) round(t0, Ragged{});
 }
 
-// Row sums (loss, k, cut, kept), weights and the result, by one block.
-__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction,
-                                              float* __restrict__ row_weight, float* __restrict__ loss,
+// What a row adds to the mean: its sums (loss, k, cut) times its own weight, 1 or 1 / its length, and its share of the
+// divisor, its length or 1.  The divisor is known last; it goes behind the rows' weights, and the backward multiplies both.
+__device__ __forceinline__ double add_row(const double (&row)[4], int reduction, double (&sum)[4]) {
+  if (!(row[3] > 0.)) return 0.;
+  const double w = reduction == MOLT_REDUCE_TOKEN ? 1. : 1. / row[3];
+  for (int i = 0; i < 3; ++i) sum[i] += w * row[i];
+  sum[3] += w * row[3];
+  return w;
+}
+
+__device__ __forceinline__ void policy_result(double (&sum)[4], float* __restrict__ scale, float* __restrict__ loss,
                                               float* __restrict__ stats) {
-  const auto row_sum = [&](long long b, double (&row)[4]) {
-    for (int i = 0; i < 4; ++i) row[i] = 0.;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s)
-      for (int i = 0; i < 4; ++i) row[i] += part[(b * splits + s) * 4 + i];
-  };
-  // a thread's first row is read once; rows beyond the block's size a second time
-  double first[4] = {0., 0., 0., 0.}, row[4];
-  double count[1] = {0.};
-  for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
-    row_sum(b, row);
-    if (b < blockDim.x)
-      for (int i = 0; i < 4; ++i) first[i] = row[i];
-    count[0] += reduction == MOLT_REDUCE_TOKEN ? row[3] : (row[3] > 0. ? 1. : 0.);
-  }
-  block_sum(count);
-  const double total = count[0];
-  double sum[3] = {0., 0., 0.};
-  for (long long b = threadIdx.x; b < batch; b += blockDim.x) {
-    if (b < blockDim.x) {
-      for (int i = 0; i < 4; ++i) row[i] = first[i];
-    } else {
-      row_sum(b, row);
-    }
-    double w = 0.;
-    if (row[3] > 0.) {
-      w = reduction == MOLT_REDUCE_TOKEN ? 1. / total : 1. / (total * row[3]);
-      for (int i = 0; i < 3; ++i) sum[i] += w * row[i];
-    }
-    if (row_weight != nullptr) row_weight[b] = (float)w;
-  }
   block_sum(sum);
   if (threadIdx.x == 0) {
-    loss[0] = (float)sum[0];
-    stats[0] = (float)sum[1];
-    stats[1] = (float)sum[2];
+    const double one = sum[3] > 0. ? 1. / sum[3] : 0.;
+    loss[0] = (float)(sum[0] * one);
+    stats[0] = (float)(sum[1] * one);
+    stats[1] = (float)(sum[2] * one);
+    if (scale != nullptr) scale[0] = (float)one;
   }
 }
 
+// Rows, their weights and the result, by one block.
+__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction,
+                                              float* __restrict__ row_weight, float* __restrict__ loss,
+                                              float* __restrict__ stats) {
+  double sum[4] = {0., 0., 0., 0.};
+  for (long long b = first_row(splits); b < batch; b += row_step(splits)) {
+    double row[4];
+    row_sums(part, b, splits, row);
+    if (speaks(splits)) {
+      const double w = add_row(row, reduction, sum);
+      if (row_weight != nullptr) row_weight[b] = (float)w;
+    }
+  }
+  policy_result(sum, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
+}
+
 template <bool REF, bool MASK>
-__global__ void __launch_bounds__(kThreads, 6) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad,
+__global__ void __launch_bounds__(kThreads, 5) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad,
                                                              double* __restrict__ part) {
   const long long b = blockIdx.x;
   const int begin = blockIdx.y * a.part;
@@ -240,6 +266,36 @@ __global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __
                                                              int reduction, float* __restrict__ row_weight,
                                                              float* __restrict__ loss, float* __restrict__ stats) {
   policy_finish(part, batch, splits, reduction, row_weight, loss, stats);
+}
+
+// A warp per row: what the block's rows add to the mean goes to part[block].
+template <bool REF, bool MASK>
+__global__ void __launch_bounds__(kThreads, 4) policy_rows_kernel(PolicyArgs a, int reduction, float* __restrict__ unit_grad,
+                                                                  float* __restrict__ row_weight, double* __restrict__ part) {
+  __shared__ double of_warp[4 * 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sum[4] = {0., 0., 0., 0.};
+  for (long long b = (long long)blockIdx.x * kWarps + warp; b < a.batch; b += (long long)gridDim.x * kWarps) {
+    Sums<2, 2> one;
+    policy_tokens<REF, MASK>(a, b, lane, a.seq, 32, unit_grad, one);
+    one.join_warp();
+    const double row[4] = {one.v[0], one.v[1], (double)one.n[0], (double)one.n[1]};
+    const double w = add_row(row, reduction, sum);
+    if (lane == 0 && row_weight != nullptr) row_weight[b] = (float)w;
+  }
+  if (lane == 0)
+    for (int i = 0; i < 4; ++i) of_warp[i * 32 + warp] = sum[i];
+  const double mine = join_block(of_warp, 4);
+  if (lane == 0 && warp < 4) part[blockIdx.x * 4 + warp] = mine;
+}
+
+__global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const double* __restrict__ part, int blocks,
+                                                                     float* __restrict__ scale, float* __restrict__ loss,
+                                                                     float* __restrict__ stats) {
+  double sum[4] = {0., 0., 0., 0.};
+  for (int k = threadIdx.x; k < blocks; k += blockDim.x)
+    for (int i = 0; i < 4; ++i) sum[i] += part[k * 4 + i];
+  policy_result(sum, scale, loss, stats);
 }
 
 // The whole forward in one block: a warp takes one of the splits of a row.
@@ -260,19 +316,55 @@ __global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs 
   policy_finish(part, a.batch, a.splits, reduction, row_weight, loss, stats);
 }
 
-// Backward passes: a block is one round of one row.
+// Backward passes.  A block is one round of one row; where rows are short (SHORT) it is one round of all tokens, numbered
+// through, and every token looks its row up (65536 x 16 tokens with a block per row: 37 us).
+constexpr int kShort = kRound / 2;
+
+struct Place {
+  long long row, token, flat;
+  bool valid;
+};
+template <bool SHORT>
+__device__ __forceinline__ Place place(long long rows, int seq, int j) {
+  Place p;
+  if (SHORT) {
+    p.flat = (long long)blockIdx.x * kRound + j * kThreads + threadIdx.x;
+    p.valid = p.flat < rows * seq;
+    // 32-bit division where it is enough
+    p.row = rows * seq <= 0xffffffffLL ? (long long)((unsigned)p.flat / (unsigned)seq) : p.flat / seq;
+    p.token = p.flat - p.row * seq;
+  } else {
+    p.row = blockIdx.x;
+    p.token = (long long)blockIdx.y * kRound + j * kThreads + threadIdx.x;
+    p.flat = p.row * seq + p.token;
+    p.valid = p.token < seq;
+  }
+  return p;
+}
+bool short_rows(int64_t rows, int64_t seq) { return seq <= kShort && (rows * seq + kRound - 1) / kRound < (1LL << 31); }
+dim3 backward_grid(int64_t rows, int64_t seq) {
+  return short_rows(rows, seq) ? dim3((unsigned)((rows * seq + kRound - 1) / kRound))
+                               : dim3((unsigned)rows, (unsigned)((seq + kRound - 1) / kRound));
+}
+
+template <bool SHORT>
 __global__ void __launch_bounds__(kThreads) policy_backward_kernel(const float* __restrict__ unit_grad,
                                                                    const float* __restrict__ row_weight,
                                                                    const float* __restrict__ grad_loss,
-                                                                   float* __restrict__ grad_logprob, long long seq) {
-  const long long b = blockIdx.x, first = b * seq, t0 = (long long)blockIdx.y * kRound + threadIdx.x;
-  float u[kUnroll];
+                                                                   float* __restrict__ grad_logprob, long long batch, int seq) {
+  float u[kUnroll], w[kUnroll];
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j) u[j] = t0 + j * kThreads < seq ? unit_grad[first + t0 + j * kThreads] : 0.f;
-  const float w = row_weight[b] * grad_loss[0];
+  for (int j = 0; j < kUnroll; ++j) {   // all loads before the first store
+    const Place p = place<SHORT>(batch, seq, j);
+    u[j] = p.valid ? unit_grad[p.flat] : 0.f;
+    w[j] = SHORT ? (p.valid ? row_weight[p.row] : 0.f) : row_weight[blockIdx.x];
+  }
+  const float g = row_weight[batch] * grad_loss[0];
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j)
-    if (t0 + j * kThreads < seq) grad_logprob[first + t0 + j * kThreads] = u[j] == 0.f ? 0.f : u[j] * w;
+  for (int j = 0; j < kUnroll; ++j) {
+    const Place p = place<SHORT>(batch, seq, j);
+    if (p.valid) grad_logprob[p.flat] = u[j] == 0.f ? 0.f : u[j] * (w[j] * g);
+  }
 }
 
 // ---- preference pairs ----------------------------------------------------------------------------------------------
@@ -316,21 +408,19 @@ __device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long 
 __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const double* part, float* __restrict__ seq_grad,
                                                   float* __restrict__ rewards, float* __restrict__ loss_out) {
   double total[1] = {0.};
-  for (long long p = threadIdx.x; p < a.pairs; p += blockDim.x) {
+  for (long long p = first_row(a.splits); p < a.pairs; p += row_step(a.splits)) {
     double s[2], scale[2];
     for (int side = 0; side < 2; ++side) {
       const long long i = p + side * a.pairs;
-      double sum = 0., kept = 0.;
-#pragma unroll 4
-      for (int k = 0; k < a.splits; ++k) {
-        sum += part[(i * a.splits + k) * 2];
-        kept += part[(i * a.splits + k) * 2 + 1];
-      }
+      double row[2];
+      row_sums(part, i, a.splits, row);
+      const double sum = row[0], kept = row[1];
       scale[side] = a.average ? (kept > 0. ? 1. / kept : 0.) : 1.;
       s[side] = a.average ? (kept > 0. ? sum / kept : 0.) : sum;
       if (a.ref != nullptr && !a.ref_per_token) s[side] -= (double)a.ref[i * a.ref_stride];
-      rewards[i] = (float)(a.beta * s[side]);
+      if (speaks(a.splits)) rewards[i] = (float)(a.beta * s[side]);
     }
+    if (!speaks(a.splits)) continue;
     const double h = s[0] - s[1];
     double loss, slope;
     if (a.kind == MOLT_PREFERENCE_SIGMOID) {
@@ -372,6 +462,18 @@ __global__ void __launch_bounds__(kThreads, 8) preference_kernel(PreferenceArgs 
   if ((threadIdx.x & 31) == 0 && value < 2) part[(i * a.splits + blockIdx.y) * 2 + value] = mine;
 }
 
+// A warp per row.
+template <bool REF, bool MASK>
+__global__ void __launch_bounds__(kThreads, 8) preference_rows_kernel(PreferenceArgs a, double* __restrict__ part) {
+  const int lane = threadIdx.x & 31;
+  for (long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); i < 2 * a.pairs; i += (long long)gridDim.x * kWarps) {
+    Sums<1, 1> sum;
+    preference_tokens<REF, MASK>(a, i, lane, a.seq, 32, sum);
+    sum.join_warp();
+    if (lane == 0) sum.store(part + i * 2, 1);
+  }
+}
+
 __global__ void __launch_bounds__(kFinish) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
                                                                  float* __restrict__ seq_grad, float* __restrict__ rewards,
                                                                  float* __restrict__ loss) {
@@ -394,19 +496,24 @@ __global__ void __launch_bounds__(kOneBlock) preference_one_block_kernel(Prefere
   preference_finish(a, part, seq_grad, rewards, loss);
 }
 
+template <bool SHORT>
 __global__ void __launch_bounds__(kThreads) preference_backward_kernel(const uint8_t* __restrict__ mask, long long mask_stride,
                                                                        const float* __restrict__ seq_grad,
                                                                        const float* __restrict__ grad_loss,
-                                                                       float* __restrict__ grad_logprob, long long seq) {
-  const long long i = blockIdx.x, t0 = (long long)blockIdx.y * kRound + threadIdx.x;
-  bool kept[kUnroll];
+                                                                       float* __restrict__ grad_logprob, long long rows, int seq) {
+  const float one = SHORT ? 0.f : seq_grad[blockIdx.x], g = grad_loss[0];
+  float w[kUnroll];
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j)
-    kept[j] = t0 + j * kThreads < seq && (mask == nullptr || mask[i * mask_stride + t0 + j * kThreads] != 0);
-  const float g = seq_grad[i] * grad_loss[0];
+  for (int j = 0; j < kUnroll; ++j) {   // all loads before the first store
+    const Place p = place<SHORT>(rows, seq, j);
+    const float of_row = SHORT ? (p.valid ? seq_grad[p.row] : 0.f) : one;
+    w[j] = p.valid && (mask == nullptr || mask[p.row * mask_stride + p.token] != 0) ? of_row : 0.f;
+  }
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j)
-    if (t0 + j * kThreads < seq) grad_logprob[i * seq + t0 + j * kThreads] = kept[j] ? g : 0.f;
+  for (int j = 0; j < kUnroll; ++j) {
+    const Place p = place<SHORT>(rows, seq, j);
+    if (p.valid) grad_logprob[p.flat] = w[j] == 0.f ? 0.f : w[j] * g;
+  }
 }
 
 int check_sizes(const char* who, int64_t rows, int64_t seq) {
@@ -427,7 +534,7 @@ using namespace molt;
 
 extern "C" size_t molt_policy_loss_workspace_bytes(int64_t batch, int64_t seq) {
   if (batch <= 0 || seq < 0 || one_block(batch, seq)) return 0;
-  return (size_t)batch * splits_for(batch, seq) * 4 * sizeof(double);
+  return (warp_rows(batch, seq) ? (size_t)warp_row_blocks(batch) : (size_t)batch * splits_for(batch, seq)) * 4 * sizeof(double);
 }
 
 extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logprob, const float* ref_logprob,
@@ -471,6 +578,15 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
     return launch_status("policy_one_block_kernel");
   }
   auto* part = reinterpret_cast<double*>(workspace);
+  if (warp_rows(batch, seq)) {
+    const int blocks = warp_row_blocks(batch);
+    const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_rows_kernel<true, true> : policy_rows_kernel<true, false>)
+                                               : (mask != nullptr ? policy_rows_kernel<false, true> : policy_rows_kernel<false, false>);
+    kernel<<<blocks, kThreads, 0, s>>>(a, reduction, unit_grad, row_weight, part);
+    if (int rc = launch_status("policy_rows_kernel")) return rc;
+    policy_rows_finish_kernel<<<1, kFinish, 0, s>>>(part, blocks, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
+    return launch_status("policy_rows_finish_kernel");
+  }
   const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_kernel<true, true> : policy_kernel<true, false>)
                                              : (mask != nullptr ? policy_kernel<false, true> : policy_kernel<false, false>);
   kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
@@ -485,15 +601,15 @@ extern "C" int molt_policy_loss_bwd(const float* unit_grad, const float* row_wei
   if (int rc = check_sizes(who, batch, seq)) return rc;
   if (batch == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(unit_grad && row_weight && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
-  const dim3 grid((unsigned)batch, (unsigned)((seq + kRound - 1) / kRound));
-  policy_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(unit_grad, row_weight, grad_loss, grad_logprob,
-                                                                                       seq);
+  const auto kernel = short_rows(batch, seq) ? policy_backward_kernel<true> : policy_backward_kernel<false>;
+  kernel<<<backward_grid(batch, seq), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(unit_grad, row_weight, grad_loss,
+                                                                                            grad_logprob, batch, (int)seq);
   return launch_status("policy_backward_kernel");
 }
 
 extern "C" size_t molt_preference_loss_workspace_bytes(int64_t pairs, int64_t seq) {
   if (pairs <= 0 || seq < 0 || one_block(2 * pairs, seq)) return 0;
-  return (size_t)pairs * 2 * splits_for(pairs * 2, seq) * 2 * sizeof(double);
+  return (size_t)pairs * 2 * (warp_rows(2 * pairs, seq) ? 1 : splits_for(pairs * 2, seq)) * 2 * sizeof(double);
 }
 
 extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_logprob, int ref_per_token, const uint8_t* mask,
@@ -531,6 +647,15 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
     return launch_status("preference_one_block_kernel");
   }
   auto* part = reinterpret_cast<double*>(workspace);
+  if (warp_rows(2 * pairs, seq)) {
+    a.splits = 1;
+    const auto kernel = tokens ? (mask != nullptr ? preference_rows_kernel<true, true> : preference_rows_kernel<true, false>)
+                               : (mask != nullptr ? preference_rows_kernel<false, true> : preference_rows_kernel<false, false>);
+    kernel<<<warp_row_blocks(2 * pairs), kThreads, 0, s>>>(a, part);
+    if (int rc = launch_status("preference_rows_kernel")) return rc;
+    preference_finish_kernel<<<1, kFinish, 0, s>>>(a, part, seq_grad, rewards, loss);
+    return launch_status("preference_finish_kernel");
+  }
   const auto kernel = tokens ? (mask != nullptr ? preference_kernel<true, true> : preference_kernel<true, false>)
                              : (mask != nullptr ? preference_kernel<false, true> : preference_kernel<false, false>);
   kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
@@ -547,8 +672,8 @@ extern "C" int molt_preference_loss_bwd(const uint8_t* mask, int64_t mask_stride
   if (pairs == 0 || seq == 0) return MOLT_OK;
   MOLT_REQUIRE(seq_grad && grad_loss && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   if (int rc = check_stride(who, "mask", mask_stride, seq)) return rc;
-  const dim3 grid((unsigned)(2 * pairs), (unsigned)((seq + kRound - 1) / kRound));
-  preference_backward_kernel<<<grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(mask, mask_stride, seq_grad, grad_loss,
-                                                                                           grad_logprob, seq);
+  const auto kernel = short_rows(2 * pairs, seq) ? preference_backward_kernel<true> : preference_backward_kernel<false>;
+  kernel<<<backward_grid(2 * pairs, seq), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      mask, mask_stride, seq_grad, grad_loss, grad_logprob, 2 * pairs, (int)seq);
   return launch_status("preference_backward_kernel");
 }

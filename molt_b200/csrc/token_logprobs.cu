@@ -59,7 +59,6 @@ struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int kElements = 4;
-  static constexpr unsigned kMinusInf = 0xff800000u;
   static __device__ __forceinline__ float largest(const uint4& q, float m) {
     return fmaxf(fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w))), m);
   }
@@ -81,7 +80,6 @@ struct Vec<float> {
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int kElements = 8;
-  static constexpr unsigned kMinusInf = 0xff80ff80u;
   static __device__ __forceinline__ unsigned max2(unsigned a, unsigned b) {   // drops a NaN, which the sum then carries
     unsigned r;
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -564,7 +562,7 @@ int launch_clusters(const char* what, void (*kernel)(Params...), int64_t rows, i
 
 // Threads for a row of `vectors` 16-byte vectors.  A block that is done too soon spends its time on being launched, on its
 // first loads and on its join: it is made as small as leaves a thread 13 vectors (16384 rows x 8192 bf16, forward: 99 us with
-// 512 threads, SMALL with 64), but not so small that there are too few threads for the device (while a thread keeps 4).
+// 512 threads, 46 with 64), but not so small that there are too few threads for the device (while a thread keeps 4).
 int threads_for(int64_t rows, int64_t vectors, int most, int resident) {
   int threads = 64;
   while (threads < most && vectors >= 2 * threads * 13) threads *= 2;

@@ -68,7 +68,7 @@ def _row_stride(tensor: Optional[torch.Tensor]) -> int:
 
 
 def _policy_forward(call, trained: bool):
-    """Loss, ``[k, cut]`` and, for the backward pass, the gradients per token with the weights per sequence behind them."""
+    """Loss, ``[k, cut]`` and, for the backward pass, the gradients per token with the weights behind them."""
     lp, old, ref, advantages, mask, clip_low, clip_high, kl_coef, reduction = call
     lp, old, ref, mask, advantages = _rows(lp), _rows(old), _rows(ref), _rows(mask), _rows(advantages)
     batch, seq = lp.shape
@@ -76,7 +76,7 @@ def _policy_forward(call, trained: bool):
     loss, stats = lp.new_empty(()), lp.new_empty(2)
     kept, unit, weight = None, None, None
     if trained:
-        kept = lp.new_empty(batch * seq + batch)
+        kept = lp.new_empty(batch * seq + batch + 1)
         unit = kept.data_ptr()
         weight = unit + 4 * batch * seq
     lib = _native.library()

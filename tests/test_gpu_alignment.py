@@ -322,7 +322,8 @@ def test_token_logprob_gradient_against_differences(native_library):
 # A token's ratio is off by 2^-22 (exp) + |d| u, its products by u each; k and 1 - exp(e) by less than 8u relatively (the
 # difference e is off by u |e|, which moves k by 2u and 1 - exp(e) by (1 + |e|) u, |e| < 5): 16u = 2^-20 of the terms'
 # magnitudes covers both.  Sums are held in 64 bits; every output is rounded once (u) and weights are rounded (u).
-POLICY_CASES = [(1, 1), (1, 7), (3, 16), (4, 64), (5, 257), (2, 4099), (64, 100), (700, 33), (1, 70001), (2000, 1)]
+POLICY_CASES = [(1, 1), (1, 7), (3, 16), (4, 64), (5, 257), (2, 4099), (64, 100), (257, 31), (700, 33), (1, 70001), (2000, 1),
+                (2047, 40), (2048, 40), (3001, 1), (2049, 1024), (2050, 1025), (12000, 17), (3, 513), (20, 512), (1, 1_300_000)]
 
 
 def _policy_inputs(batch, seq, gen, per_token, ragged):
@@ -495,7 +496,7 @@ def test_policy_loss_strides_masks_and_refusals(native_library):
 # ---- preference loss -----------------------------------------------------------------------------------------------
 # The differences of a sequence are each off by u at most before they are added in 64 bits: s by 2u sum |lp - ref| (twice what
 # is needed, for the rounding of the reward), the loss by its slope times the errors of both sums, and a rounding.
-PAIR_CASES = [(1, 1), (2, 129), (3, 1000), (40, 77), (1, 100003), (600, 3)]
+PAIR_CASES = [(1, 1), (2, 129), (3, 1000), (40, 77), (1, 100003), (600, 3), (1023, 50), (1024, 50), (1025, 1025), (5000, 9), (1, 700_001)]
 
 
 @pytest.mark.parametrize("pairs,seq", PAIR_CASES)
