@@ -319,9 +319,10 @@ int molt_mlp_bwd_t(const molt_lora_proj* gate, const molt_lora_proj* up, const m
 
 /* Log-probability of one given token per row of logits [rows, vocab] (dtype MOLT_DTYPE_BF16 or MOLT_DTYPE_F32; row r begins
  * row_stride * r elements behind the first, row_stride 0 reads one row for all):
- *   logprob[r] = (x[t] - max) / T - ln(sum_v exp((x[v] - max) / T)),   t = token_ids[r], T = temperature.
+ *   logprob[r] = (x[t] - max) / T - ln(sum_v exp((x[v] - max) / T)),   t = token_ids[r], T = temperature,
+ * 1e-30 <= T <= 1e30.
  * A token id outside [0, vocab) (an ignore index such as -100) gives 0 and its row is not read.  Logits of -inf have
- * probability zero; a row without a finite logit, or with NaN or +inf, gives NaN.  stats (optional): [rows, 2] floats
+ * probability zero; a row without a finite logit, or with NaN or +inf, gives NaN.  stats (optional): [rows, 2] floats, 8-byte aligned,
  * for molt_token_logprob_bwd (what the exponents were taken from, and log2 of the sum).  fp32 arithmetic. */
 int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, float temperature,
                            float* logprob, float* stats, int64_t rows, int64_t vocab, uintptr_t stream);

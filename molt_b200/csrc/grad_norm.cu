@@ -165,6 +165,8 @@ __device__ __forceinline__ double chunk_total(const T* g, int n, double acc) {
   return acc;
 }
 
+// HBM-bound: 742 MB in 84 tensors take 112 us (6.6 TB/s), a 74 MB arena 14.7 us.  8 loads in flight per thread, 4096 or 16384
+// elements per chunk and more blocks were each within 5 %, or slower.
 template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 5) norm_kernel(const __grid_constant__ Table<CAPACITY> table,
                                                         double* __restrict__ part) {
@@ -231,7 +233,8 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int n, float c) 
 }
 
 // Every block adds the partial sums up for itself (they lie in the L2) instead of waiting for one that does.  The chunks
-// are taken from the last to the first: what the norm read last is what the L2 still holds.
+// are taken from the last to the first: what the norm read last is what the L2 still holds.  HBM-bound: 742 MB read and
+// written take 220 us (6.7 TB/s), the 74 MB arena 22 us.
 template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
                                                          const double* __restrict__ part, int parts, float max_norm,

@@ -1,7 +1,11 @@
 // Losses over token log-probabilities: the clipped policy loss with a KL term, and the loss over preference pairs.
-// All of it is one pass over a few fp32 arrays of [batch, seq] (HBM- or, for small batches, launch-bound).  The weights
-// of the mean are only known once all masks have been counted, and the scale of the gradient arrives with the backward
-// pass, so the forward writes the gradient without either and the backward multiplies both in.
+// One pass over a few fp32 arrays of [batch, seq].  The weights of the mean are only known once all masks have been counted,
+// and the scale of the gradient arrives with the backward pass, so the forward writes the gradient without either and the
+// backward multiplies both in (29 bytes per token in all with a reference; recomputing in the backward would move 38).
+// What bounds them: small batches the launches (one for a forward of at most 8192 tokens, 6.5 us; 3 us for a backward);
+// 512 x 4096 tokens the arithmetic of about 125 instructions per token and the latency of one wave of blocks (policy forward
+// 15 us where the bytes would take 5, preference forward 11 us for twice the tokens); 2048 x 4096 tokens HBM to about a half
+// (46 us policy, 17 us preference, 9-11 us backward).
 #include <math.h>
 
 #include <type_traits>
@@ -129,21 +133,40 @@ struct PolicyArgs {
   long long batch;
   int seq, per_token, splits, part;   // part: tokens of one of the splits of a row
   double log_high, log_low;   // ln(1 + clip_high), ln(1 - clip_low): the borders of ln r
-  float log_high_f, log_low_f, high, low, kl_coef;   // the borders rounded to fp32; 1 + clip_high, 1 - clip_low
+  float log_high_f, log_low_f, above, below, kl_coef;   // the borders rounded to fp32; the clamp's ends less one
 };
 
-// exp(d) - 1 - d without the cancellation: the Taylor series d^2 (1/2! + d (1/3! + d (1/4! + ...))) for |d| <= 1, to the term
-// d^12 (what it leaves out is below 2/13! < 2^-31 of the result), the plain difference elsewhere.  One range for nearly all
-// tokens of a policy near its reference, so that a warp seldom takes both ways.
-__device__ __forceinline__ float exp_minus_1_minus(float d) {
-  if (d > 60.f) return expf(d);   // 1 + d is below its last bit; an infinite d must not meet itself
-  if (fabsf(d) > 1.f) return expm1f(d) - d;
+// (exp(d) - 1 - d) / d^2 for |d| <= 1: the Taylor series 1/2! + d (1/3! + d (1/4! + ...)) to the term d^12 of the exponential;
+// what it leaves out is below 2/13! < 2^-31 of the result.  Nearly all tokens of a policy near the one that sampled, and near
+// its reference, lie in this range, so that a warp seldom takes the other way as well.
+__device__ __forceinline__ float exp_tail(float d) {
   constexpr float kInverseFactorial[] = {1.f / 2, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320, 1.f / 362880,
                                          1.f / 3628800, 1.f / 39916800, 1.f / 479001600};
   float r = kInverseFactorial[10];
 #pragma unroll
   for (int k = 9; k >= 0; --k) r = fmaf(r, d, kInverseFactorial[k]);
-  return d * d * r;
+  return r;
+}
+// r = exp(d) and less = r - 1, both to a few roundings of their own size.
+__device__ __forceinline__ void ratio(float d, float& r, float& less) {
+  if (fabsf(d) <= 1.f) {
+    less = fmaf(d * d, exp_tail(d), d);
+    r = 1.f + less;
+  } else {
+    r = expf(d);
+    less = r - 1.f;
+  }
+}
+// k = exp(d) - 1 - d and slope = exp(d) - 1.
+__device__ __forceinline__ void divergence(float d, float& k, float& slope) {
+  if (fabsf(d) <= 1.f) {
+    const float tail = exp_tail(d);
+    k = d * d * tail;
+    slope = fmaf(d * d, tail, d);
+  } else {
+    slope = expm1f(d);
+    k = d > 60.f ? slope : slope - d;   // 1 + d is below the last bit; an infinite d must not meet itself
+  }
 }
 
 // Tokens begin, begin + step, ... below end of row b, kUnroll of them loaded at a time; full rounds need no bounds checks.
@@ -171,6 +194,7 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
       kept[j] = (FULL || t0 + j * step < end) && (!MASK || mask_row[t] != 0);
     }
     float loss = 0.f, ks = 0.f;
+    double level = 0.;
     int cuts = 0, keeps = 0;
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
@@ -181,25 +205,27 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
         const double exact = (double)lp[j] - (double)old[j];
         cut = (adv[j] > 0.f && exact > a.log_high) || (adv[j] < 0.f && exact < a.log_low);
       }
-      const float r = expf(d);
-      // the product with an advantage of zero is zero however large the ratio (NaN stays NaN)
-      float l = adv[j] == 0.f ? 0.f : -(cut ? (adv[j] > 0.f ? a.high : a.low) : r) * adv[j];
+      float r, less;
+      ratio(d, r, less);
+      // -r A as -A, added in 64 bits, and -(r - 1) A, which is small near the policy that sampled: advantages of both signs
+      // cancel in the mean, the rounding of products of order one would not.  The product with an advantage of zero is zero
+      // however large the ratio (NaN stays NaN).
+      const float rest = adv[j] == 0.f ? 0.f : -(cut ? (adv[j] > 0.f ? a.above : a.below) : less) * adv[j];
       float g = cut || adv[j] == 0.f ? 0.f : -r * adv[j];
       if (REF) {
-        const float e = ref[j] - lp[j], k = exp_minus_1_minus(e);
-        if (a.kl_coef != 0.f) {
-          l += a.kl_coef * k;
-          g -= a.kl_coef * (k + e);   // exp(e) - 1
-        }
+        float k, slope;
+        divergence(ref[j] - lp[j], k, slope);
+        if (a.kl_coef != 0.f) g -= a.kl_coef * slope;
         ks += kept[j] ? k : 0.f;
       }
-      loss += kept[j] ? l : 0.f;
+      loss += kept[j] ? rest : 0.f;
+      level -= kept[j] ? (double)adv[j] : 0.;
       cuts += kept[j] && cut;
       keeps += kept[j];
       if (unit_row != nullptr && (FULL || t0 + j * step < end)) unit_row[t0 + j * step] = kept[j] ? g : 0.f;
     }
-    // four tokens in fp32, then in 64 bits: three roundings more on values that carry a few already
-    sum.v[0] += loss;
+    // the small parts of four tokens in fp32, then in 64 bits
+    sum.v[0] += level + (double)loss;
     if (REF) sum.v[1] += ks;
     sum.n[0] += cuts;
     sum.n[1] += keeps;
@@ -219,12 +245,12 @@ __device__ __forceinline__ double add_row(const double (&row)[4], int reduction,
   return w;
 }
 
-__device__ __forceinline__ void policy_result(double (&sum)[4], float* __restrict__ scale, float* __restrict__ loss,
-                                              float* __restrict__ stats) {
+__device__ __forceinline__ void policy_result(double (&sum)[4], double kl_coef, float* __restrict__ scale,
+                                              float* __restrict__ loss, float* __restrict__ stats) {
   block_sum(sum);
   if (threadIdx.x == 0) {
     const double one = sum[3] > 0. ? 1. / sum[3] : 0.;
-    loss[0] = (float)(sum[0] * one);
+    loss[0] = (float)((kl_coef != 0. ? sum[0] + kl_coef * sum[1] : sum[0]) * one);
     stats[0] = (float)(sum[1] * one);
     stats[1] = (float)(sum[2] * one);
     if (scale != nullptr) scale[0] = (float)one;
@@ -232,7 +258,7 @@ __device__ __forceinline__ void policy_result(double (&sum)[4], float* __restric
 }
 
 // Rows, their weights and the result, by one block.
-__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction,
+__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction, double kl_coef,
                                               float* __restrict__ row_weight, float* __restrict__ loss,
                                               float* __restrict__ stats) {
   double sum[4] = {0., 0., 0., 0.};
@@ -244,7 +270,7 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
       if (row_weight != nullptr) row_weight[b] = (float)w;
     }
   }
-  policy_result(sum, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
+  policy_result(sum, kl_coef, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
 }
 
 template <bool REF, bool MASK>
@@ -263,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 5) policy_kernel(PolicyArgs a, float
 }
 
 __global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
-                                                             int reduction, float* __restrict__ row_weight,
+                                                             int reduction, double kl_coef, float* __restrict__ row_weight,
                                                              float* __restrict__ loss, float* __restrict__ stats) {
-  policy_finish(part, batch, splits, reduction, row_weight, loss, stats);
+  policy_finish(part, batch, splits, reduction, kl_coef, row_weight, loss, stats);
 }
 
 // A warp per row: what the block's rows add to the mean goes to part[block].
@@ -289,18 +315,19 @@ __global__ void __launch_bounds__(kThreads, 4) policy_rows_kernel(PolicyArgs a, 
   if (lane == 0 && warp < 4) part[blockIdx.x * 4 + warp] = mine;
 }
 
-__global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const double* __restrict__ part, int blocks,
+__global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const double* __restrict__ part, int blocks, double kl_coef,
                                                                      float* __restrict__ scale, float* __restrict__ loss,
                                                                      float* __restrict__ stats) {
   double sum[4] = {0., 0., 0., 0.};
   for (int k = threadIdx.x; k < blocks; k += blockDim.x)
     for (int i = 0; i < 4; ++i) sum[i] += part[k * 4 + i];
-  policy_result(sum, scale, loss, stats);
+  policy_result(sum, kl_coef, scale, loss, stats);
 }
 
 // The whole forward in one block: a warp takes one of the splits of a row.
 template <bool REF, bool MASK>
-__global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs a, int reduction, float* __restrict__ unit_grad,
+__global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs a, int reduction, double kl_coef,
+                                                                     float* __restrict__ unit_grad,
                                                                      float* __restrict__ row_weight, float* __restrict__ loss,
                                                                      float* __restrict__ stats) {
   __shared__ double part[kOneBlockRows * 4];
@@ -313,7 +340,7 @@ __global__ void __launch_bounds__(kOneBlock) policy_one_block_kernel(PolicyArgs 
     if (lane == 0) sum.store(part + u * 4, 1);
   }
   __syncthreads();
-  policy_finish(part, a.batch, a.splits, reduction, row_weight, loss, stats);
+  policy_finish(part, a.batch, a.splits, reduction, kl_coef, row_weight, loss, stats);
 }
 
 // Backward passes.  A block is one round of one row; where rows are short (SHORT) it is one round of all tokens, numbered
@@ -385,19 +412,20 @@ __device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long 
   const uint8_t* mask_row = MASK ? a.mask + i * a.mask_stride : nullptr;
   const auto round = [&](int t0, auto full) {
     constexpr bool FULL = decltype(full)::value;
-    float d[kUnroll];
+    float lp[kUnroll], ref[kUnroll];
     bool kept[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const int t = FULL || t0 + j * step < end ? t0 + j * step : t0;   // a token of the row in any case
-      d[j] = REF ? lp_row[t] - ref_row[t] : lp_row[t];
+      lp[j] = lp_row[t];
+      if (REF) ref[j] = ref_row[t];
       kept[j] = (FULL || t0 + j * step < end) && (!MASK || mask_row[t] != 0);
     }
 #pragma unroll
-    for (int j = 0; j < kUnroll; j += 2) {
-      // a pair of fp32 differences is added before it goes on in 64 bits: two roundings of the terms' magnitudes
-      sum.v[0] += (kept[j] ? d[j] : 0.f) + (kept[j + 1] ? d[j + 1] : 0.f);
-      sum.n[0] += (int)kept[j] + (int)kept[j + 1];
+    for (int j = 0; j < kUnroll; ++j) {
+      // in 64 bits from the start: the differences of a sequence cancel, their rounding would not
+      if (kept[j]) sum.v[0] += REF ? (double)lp[j] - (double)ref[j] : (double)lp[j];
+      sum.n[0] += kept[j];
     }
   };
   int t0 = begin;
@@ -567,14 +595,14 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
   a.splits = splits_for(batch, seq); a.part = part_tokens(batch, seq);
   a.log_high = log1p(clip_high); a.log_low = log1p(-clip_low);
   a.log_high_f = (float)a.log_high; a.log_low_f = (float)a.log_low;
-  a.high = (float)(1. + clip_high); a.low = (float)(1. - clip_low); a.kl_coef = (float)kl_coef;
+  a.above = (float)clip_high; a.below = (float)-clip_low; a.kl_coef = (float)kl_coef;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (needed == 0) {
     a.splits = one_block_splits(batch);
     a.part = ((int)seq + a.splits - 1) / a.splits;
     const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_one_block_kernel<true, true> : policy_one_block_kernel<true, false>)
                                                : (mask != nullptr ? policy_one_block_kernel<false, true> : policy_one_block_kernel<false, false>);
-    kernel<<<1, kOneBlock, 0, s>>>(a, reduction, unit_grad, row_weight, loss, stats);
+    kernel<<<1, kOneBlock, 0, s>>>(a, reduction, kl_coef, unit_grad, row_weight, loss, stats);
     return launch_status("policy_one_block_kernel");
   }
   auto* part = reinterpret_cast<double*>(workspace);
@@ -584,14 +612,14 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
                                                : (mask != nullptr ? policy_rows_kernel<false, true> : policy_rows_kernel<false, false>);
     kernel<<<blocks, kThreads, 0, s>>>(a, reduction, unit_grad, row_weight, part);
     if (int rc = launch_status("policy_rows_kernel")) return rc;
-    policy_rows_finish_kernel<<<1, kFinish, 0, s>>>(part, blocks, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
+    policy_rows_finish_kernel<<<1, kFinish, 0, s>>>(part, blocks, kl_coef, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
     return launch_status("policy_rows_finish_kernel");
   }
   const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_kernel<true, true> : policy_kernel<true, false>)
                                              : (mask != nullptr ? policy_kernel<false, true> : policy_kernel<false, false>);
   kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
   if (int rc = launch_status("policy_kernel")) return rc;
-  policy_finish_kernel<<<1, kFinish, 0, s>>>(part, batch, a.splits, reduction, row_weight, loss, stats);
+  policy_finish_kernel<<<1, kFinish, 0, s>>>(part, batch, a.splits, reduction, kl_coef, row_weight, loss, stats);
   return launch_status("policy_finish_kernel");
 }
 

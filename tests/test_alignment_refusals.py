@@ -29,6 +29,7 @@ def _refused(code, expected, word):
     ({"dtype": 2}, _native.E_CAPABILITY, "bf16 or fp32"), ({"temperature": 0.0}, _native.E_VALUE, "temperature"),
     ({"temperature": -1.0}, _native.E_VALUE, "temperature"), ({"temperature": float("nan")}, _native.E_VALUE, "temperature"),
     ({"temperature": float("inf")}, _native.E_VALUE, "temperature"), ({"temperature": 1e-39}, _native.E_VALUE, "temperature"),
+    ({"temperature": 1e38}, _native.E_VALUE, "temperature"), ({"ids": B + 4}, _native.E_VALUE, "aligned"),
     ({"logits": None}, _native.E_VALUE, "NULL"), ({"ids": None}, _native.E_VALUE, "NULL"),
     ({"logprob": None}, _native.E_VALUE, "NULL"), ({"stride": 99}, _native.E_VALUE, "overlap"),
     ({"logits": A + 1}, _native.E_VALUE, "aligned"), ({"grad": None}, _native.E_VALUE, "NULL"),
@@ -50,6 +51,12 @@ def test_token_logprob_refusals(native_library, change, expected, word):
     if not set(change) & {"grad", "grad_stride"}:
         _refused(lib.molt_token_logprob_fwd(c["logits"], c["dtype"], c["stride"], c["ids"], c["temperature"], c["logprob"], None,
                                             c["rows"], c["vocab"], 0), expected, word)
+
+
+def test_token_logprob_stats_are_aligned(native_library):
+    lib = native_library
+    _refused(lib.molt_token_logprob_fwd(A, 0, 100, B, 1.0, D, E + 4, 4, 100, 0), _native.E_VALUE, "stats")
+    _refused(lib.molt_token_logprob_bwd(A, 0, 100, B, E + 4, E, 1.0, C, 100, 4, 100, 0), _native.E_VALUE, "stats")
 
 
 def test_token_logprob_of_no_rows_is_no_launch(native_library):

@@ -218,6 +218,15 @@ def test_token_logprobs_at_the_borders_of_their_blocks(native_library, vectors, 
         _check_all_forms(logits, ids, 0.9)
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 1e-4, 1e4, 1e30])
+@pytest.mark.parametrize("vocab", [900, 60_000])
+def test_token_logprobs_at_extreme_temperatures(native_library, temperature, vocab):
+    gen = _gen(vocab)
+    for dtype in (torch.bfloat16, torch.float32):
+        logits = (torch.randn(5, vocab, device="cuda", generator=gen) * 4).to(dtype)
+        _check_all_forms(logits, torch.randint(0, vocab, (5,), device="cuda", generator=gen), temperature)
+
+
 @pytest.mark.parametrize("rows,vocab,dtype", [(2, 700_001, torch.bfloat16), (2, 1_300_000, torch.float32), (70_000, 5, torch.float32),
                                               (66_000, 131, torch.bfloat16)])
 def test_token_logprobs_of_long_rows_and_many_rows(native_library, rows, vocab, dtype):
