@@ -274,16 +274,17 @@ _ITEM_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
 
 
 def grad_items(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]] = None) -> array:
-    """``molt_grad_item`` records (four 64-bit fields each) of a list of gradients and, when clipping, their outputs."""
+    """``molt_grad_item`` records (four 64-bit fields each) of a list of gradients and, when clipping, their outputs.  Fills
+    whole columns at a time: there may be hundreds of tensors."""
+    dtypes = [t.dtype for t in grads]
+    if not _ITEM_DTYPES.keys() >= set(dtypes):
+        raise CapabilityError("gradient norms support bfloat16 and float32 tensors")
     flat = [0] * (4 * len(grads))
-    flat[0::4] = map(torch.Tensor.data_ptr, grads)
+    flat[0::4] = list(map(torch.Tensor.data_ptr, grads))
     if outs is not None:
-        flat[1::4] = flat[0::4] if outs is grads else map(torch.Tensor.data_ptr, outs)
-    flat[2::4] = map(torch.Tensor.numel, grads)
-    try:
-        flat[3::4] = [_ITEM_DTYPES[t.dtype] for t in grads]
-    except KeyError:
-        raise CapabilityError("gradient norms support bfloat16 and float32 tensors") from None
+        flat[1::4] = flat[0::4] if outs is grads else list(map(torch.Tensor.data_ptr, outs))
+    flat[2::4] = list(map(torch.Tensor.numel, grads))
+    flat[3::4] = list(map(_ITEM_DTYPES.__getitem__, dtypes))
     return array("q", flat)
 
 

@@ -25,13 +25,15 @@ def _dense(tensor: torch.Tensor) -> bool:
     return True
 
 
-def _checked(name: str, tensors: Grads) -> Tuple[torch.Tensor, ...]:
+def _checked(name: str, tensors: Grads) -> Tuple[Tuple[torch.Tensor, ...], bool]:
+    """The tensors as a tuple, and whether all of them are contiguous; raises for one that has gaps or repeats elements."""
     tensors = (tensors,) if isinstance(tensors, torch.Tensor) else tuple(tensors)
     if not tensors:
         raise ValueError(f"{name}: at least one tensor is needed")
-    if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.numel() == 0 or _dense(t) for t in tensors):
+    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+    if not contiguous and not all(t.numel() == 0 or _dense(t) for t in tensors):
         raise ValueError(f"{name}: every tensor must fill its memory (no gaps, no repeated elements)")
-    return tensors
+    return tensors, contiguous
 
 
 def _norm_kind(norm_type: float) -> int:
@@ -69,25 +71,29 @@ def global_grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
     device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  It is right for every
     finite gradient, however large or small; a NaN gives NaN, and an infinity infinity.  Equal lists give equal bits.
     Nothing is recorded for autograd."""
-    grads = _checked("grads", grads)
+    grads, _ = _checked("grads", grads)
     return _launch(grads, None, _norm_kind(norm_type), float("inf"))
 
 
 def clip_grad_norm(grads: Grads, max_norm: float, norm_type: float = 2.0, out: Optional[Grads] = None) -> torch.Tensor:
     """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return their :func:`global_grad_norm` before that.
 
-    In place, or into ``out`` (tensors like ``grads``; an output may be its own gradient but must not overlap another
-    tensor of the call).  One tensor must not stand in the list twice.  Nothing is recorded for autograd."""
-    grads = _checked("grads", grads)
+    In place, or into ``out``: tensors of the same dtypes and sizes that lie in memory as ``grads`` do (of contiguous ones the
+    shapes may differ).  An output may be its own gradient but must not overlap another tensor of the call.  One tensor must
+    not stand in the list twice.  Nothing is recorded for autograd."""
+    grads, plain = _checked("grads", grads)
     kind = _norm_kind(norm_type)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative")
-    outs = grads if out is None else _checked("out", out)
-    if outs is not grads:
-        if len(outs) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device
-                                          for o, g in zip(outs, grads)):
-            raise ValueError("out must match grads in number, shape, dtype and device")
-        if any(o.stride() != g.stride() for o, g in zip(outs, grads) if not (o.is_contiguous() and g.is_contiguous())):
+    outs = grads
+    if out is not None and out is not grads:
+        outs, plain_outs = _checked("out", out)
+        numel, get_device = torch.Tensor.numel, torch.Tensor.get_device   # whole lists at a time: there may be hundreds
+        if (list(map(numel, outs)) != list(map(numel, grads)) or list(map(get_device, outs)) != list(map(get_device, grads))
+                or [t.dtype for t in outs] != [t.dtype for t in grads]):
+            raise ValueError("out must match grads in number, size, dtype and device")
+        if not (plain and plain_outs) and any(o.shape != g.shape or o.stride() != g.stride() for o, g in zip(outs, grads)
+                                              if not (o.is_contiguous() and g.is_contiguous())):
             raise ValueError("out must lie in memory as grads do")
     norm = _launch(grads, outs, kind, float(max_norm))
     torch.autograd.graph.increment_version(outs)

@@ -703,6 +703,9 @@ def test_grad_norm_layouts_and_refusals(native_library):
     _close(clip_grad_norm([turned, channels], 0.5), want, want * 2 ** -20)
     for t, c in zip((turned, channels), copy):
         _close(t, c, c.abs() * 2 ** -19 + 1e-6 * c.abs())
+    matrix, flat = torch.randn(6, 7, device="cuda", generator=gen), torch.zeros(50, device="cuda")
+    clip_grad_norm(matrix, 1e9, out=flat[3:45])             # contiguous outputs may have other shapes
+    assert torch.equal(flat[3:45].view(6, 7), matrix) and not bool(flat[:3].any()) and not bool(flat[45:].any())
     a, b = torch.ones(8, device="cuda"), torch.ones(8, device="cuda")
     with pytest.raises(CapabilityError):
         global_grad_norm([a.half()])
