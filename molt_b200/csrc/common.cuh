@@ -93,6 +93,26 @@ __device__ __forceinline__ float load_absmax(const WeightView& w, long long blk)
   return __fadd_rn(scaled, w.offset);
 }
 
+// Programmatic dependence of two kernels in a stream: the second one's blocks are brought up while the first one ends.  The
+// first calls let_next_begin(), the second is launched by launch_behind() and calls wait_for_previous() before it reads what
+// the first wrote (all of the first has then run and can be seen).
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+inline void launch_behind(void (*kernel)(Params...), unsigned blocks, unsigned threads, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(threads);
+  config.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, args...);   // its error is picked up by launch_status
+}
+
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

@@ -170,6 +170,7 @@ __device__ __forceinline__ double chunk_total(const T* g, int n, double acc) {
 template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 5) norm_kernel(const __grid_constant__ Table<CAPACITY> table,
                                                         double* __restrict__ part) {
+  let_next_begin();   // it waits for the partial sums itself
   double acc = 0.;
   const unsigned chunks = table.first[table.count];
   for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -197,6 +198,7 @@ __device__ __forceinline__ float2 finish(const double* __restrict__ part, int pa
 template <bool MAX>
 __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* __restrict__ part, int parts, float grad_scale,
                                                                float max_norm, float* __restrict__ result) {
+  wait_for_previous();
   const float2 r = finish<MAX>(part, parts, grad_scale, max_norm);
   if (threadIdx.x == 0) {
     result[0] = r.x;
@@ -239,6 +241,7 @@ template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
                                                          const double* __restrict__ part, int parts, float max_norm,
                                                          float* __restrict__ result) {
+  wait_for_previous();
   const float2 r = finish<MAX>(part, parts, 1.f, max_norm);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     result[0] = r.x;
@@ -296,11 +299,11 @@ int launch_scale(const molt_grad_item* items, int n, int blocks, const double* p
   if (n <= kSmallTable) {
     Table<kSmallTable> table;
     fill(table, items, n);
-    scale_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+    launch_behind(scale_kernel<MAX, kSmallTable>, blocks, kThreads, s, table, part, parts, max_norm, result);
   } else {
     Table<kTable> table;
     fill(table, items, n);
-    scale_kernel<MAX><<<blocks, kThreads, 0, s>>>(table, part, parts, max_norm, result);
+    launch_behind(scale_kernel<MAX, kTable>, blocks, kThreads, s, table, part, parts, max_norm, result);
   }
   return launch_status("scale_kernel");
 }
@@ -382,8 +385,7 @@ int norm_launch(const char* who, const molt_grad_item* items, int count, int nor
     parts += blocks;
   }
   if (!clip) {
-    if (max) norm_finish_kernel<true><<<1, kThreads, 0, s>>>(part, parts, grad_scale, max_norm, result);
-    else norm_finish_kernel<false><<<1, kThreads, 0, s>>>(part, parts, grad_scale, max_norm, result);
+    launch_behind(max ? norm_finish_kernel<true> : norm_finish_kernel<false>, 1, kThreads, s, part, parts, grad_scale, max_norm, result);
     return launch_status("norm_finish_kernel");
   }
   for (int t = tables_of(count) - 1; t >= 0; --t) {

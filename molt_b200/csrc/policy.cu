@@ -276,6 +276,7 @@ __device__ __forceinline__ void policy_finish(const double* part, long long batc
 template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kThreads, 5) policy_kernel(PolicyArgs a, float* __restrict__ unit_grad,
                                                              double* __restrict__ part) {
+  let_next_begin();
   const long long b = blockIdx.x;
   const int begin = blockIdx.y * a.part;
   __shared__ double of_warp[4 * 32];
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 5) policy_kernel(PolicyArgs a, float
 __global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
                                                              int reduction, double kl_coef, float* __restrict__ row_weight,
                                                              float* __restrict__ loss, float* __restrict__ stats) {
+  wait_for_previous();
   policy_finish(part, batch, splits, reduction, kl_coef, row_weight, loss, stats);
 }
 
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __
 template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kThreads, 4) policy_rows_kernel(PolicyArgs a, int reduction, float* __restrict__ unit_grad,
                                                                   float* __restrict__ row_weight, double* __restrict__ part) {
+  let_next_begin();
   __shared__ double of_warp[4 * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum[4] = {0., 0., 0., 0.};
@@ -318,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 4) policy_rows_kernel(PolicyArgs a, 
 __global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const double* __restrict__ part, int blocks, double kl_coef,
                                                                      float* __restrict__ scale, float* __restrict__ loss,
                                                                      float* __restrict__ stats) {
+  wait_for_previous();
   double sum[4] = {0., 0., 0., 0.};
   for (int k = threadIdx.x; k < blocks; k += blockDim.x)
     for (int i = 0; i < 4; ++i) sum[i] += part[k * 4 + i];
@@ -478,6 +482,7 @@ __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const
 
 template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kThreads, 8) preference_kernel(PreferenceArgs a, double* __restrict__ part) {
+  let_next_begin();
   const long long i = blockIdx.x;
   const int begin = blockIdx.y * a.part;
   __shared__ double of_warp[2 * 32];
@@ -493,6 +498,7 @@ __global__ void __launch_bounds__(kThreads, 8) preference_kernel(PreferenceArgs 
 // A warp per row.
 template <bool REF, bool MASK>
 __global__ void __launch_bounds__(kThreads, 8) preference_rows_kernel(PreferenceArgs a, double* __restrict__ part) {
+  let_next_begin();
   const int lane = threadIdx.x & 31;
   for (long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); i < 2 * a.pairs; i += (long long)gridDim.x * kWarps) {
     Sums<1, 1> sum;
@@ -505,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 8) preference_rows_kernel(Preference
 __global__ void __launch_bounds__(kFinish) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
                                                                  float* __restrict__ seq_grad, float* __restrict__ rewards,
                                                                  float* __restrict__ loss) {
+  wait_for_previous();
   preference_finish(a, part, seq_grad, rewards, loss);
 }
 
@@ -612,14 +619,15 @@ extern "C" int molt_policy_loss_fwd(const float* logprob, const float* old_logpr
                                                : (mask != nullptr ? policy_rows_kernel<false, true> : policy_rows_kernel<false, false>);
     kernel<<<blocks, kThreads, 0, s>>>(a, reduction, unit_grad, row_weight, part);
     if (int rc = launch_status("policy_rows_kernel")) return rc;
-    policy_rows_finish_kernel<<<1, kFinish, 0, s>>>(part, blocks, kl_coef, row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
+    launch_behind(policy_rows_finish_kernel, 1, kFinish, s, part, blocks, kl_coef,
+                  row_weight != nullptr ? row_weight + batch : nullptr, loss, stats);
     return launch_status("policy_rows_finish_kernel");
   }
   const auto kernel = ref_logprob != nullptr ? (mask != nullptr ? policy_kernel<true, true> : policy_kernel<true, false>)
                                              : (mask != nullptr ? policy_kernel<false, true> : policy_kernel<false, false>);
   kernel<<<dim3((unsigned)batch, a.splits), kThreads, 0, s>>>(a, unit_grad, part);
   if (int rc = launch_status("policy_kernel")) return rc;
-  policy_finish_kernel<<<1, kFinish, 0, s>>>(part, batch, a.splits, reduction, kl_coef, row_weight, loss, stats);
+  launch_behind(policy_finish_kernel, 1, kFinish, s, part, (long long)batch, a.splits, reduction, kl_coef, row_weight, loss, stats);
   return launch_status("policy_finish_kernel");
 }
 
@@ -681,14 +689,14 @@ extern "C" int molt_preference_loss_fwd(const float* logprob, const float* ref_l
                                : (mask != nullptr ? preference_rows_kernel<false, true> : preference_rows_kernel<false, false>);
     kernel<<<warp_row_blocks(2 * pairs), kThreads, 0, s>>>(a, part);
     if (int rc = launch_status("preference_rows_kernel")) return rc;
-    preference_finish_kernel<<<1, kFinish, 0, s>>>(a, part, seq_grad, rewards, loss);
+    launch_behind(preference_finish_kernel, 1, kFinish, s, a, part, seq_grad, rewards, loss);
     return launch_status("preference_finish_kernel");
   }
   const auto kernel = tokens ? (mask != nullptr ? preference_kernel<true, true> : preference_kernel<true, false>)
                              : (mask != nullptr ? preference_kernel<false, true> : preference_kernel<false, false>);
   kernel<<<dim3((unsigned)(2 * pairs), a.splits), kThreads, 0, s>>>(a, part);
   if (int rc = launch_status("preference_kernel")) return rc;
-  preference_finish_kernel<<<1, kFinish, 0, s>>>(a, part, seq_grad, rewards, loss);
+  launch_behind(preference_finish_kernel, 1, kFinish, s, a, part, seq_grad, rewards, loss);
   return launch_status("preference_finish_kernel");
 }
 

@@ -689,6 +689,8 @@ def test_grad_norm_of_extreme_values(native_library):
                     assert math.isnan(norm) if math.isnan(bad) else norm == float("inf")
     zero = torch.zeros(100, device="cuda")
     assert float(clip_grad_norm([zero], 1.0)) == 0.0 and not bool(zero.any())
+    nothing = torch.empty(0, 7, device="cuda")
+    assert float(clip_grad_norm([nothing], 1.0)) == 0.0 and float(global_grad_norm([nothing, nothing], float("inf"))) == 0.0
 
 
 def test_grad_norm_layouts_and_refusals(native_library):
