@@ -334,7 +334,7 @@ int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, co
                            const float* grad_logprob, float temperature, void* grad_logits, int64_t grad_stride,
                            int64_t rows, int64_t vocab, uintptr_t stream);
 
-/* Both in one pass over the logits: logprob as molt_token_logprob_fwd, grad_logits as molt_token_logprob_bwd with
+/* Both in one pass over the logits: logprob as molt_token_logprob_fwd (to rounding: it adds in another order), grad_logits as molt_token_logprob_bwd with
  * grad_logprob[r] = weight[r] (weight NULL: 1).  Meant for a loss whose gradient scales rows: with weight 1 the caller
  * multiplies by dLoss/dlogprob[r] behind the head's second GEMM, where a row is the hidden width and not the vocabulary. */
 int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, const float* weight,

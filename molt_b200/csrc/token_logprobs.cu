@@ -460,15 +460,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 // between threads.  HBM-bound: 4096 x 50304 bf16 takes 124 us (6.66 TB/s), 8192 x 32000 fp32 305 us (6.9 TB/s, some of it from
 // the L2).  A block takes 4 vectors per thread of one row: no loop, many blocks, reads and writes spread evenly (a copy
 // written like this reaches 6.7 TB/s, one with a fixed grid that loops 6.0).  Rows of ignored ids are only cleared.
-constexpr int kBackThreads = 256, kBackVectors = 4;
+constexpr int kBackVectors = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits, long long row_stride,
-                                                                const long long* __restrict__ ids,
-                                                                const float2* __restrict__ stats,
-                                                                const float* __restrict__ grad_logprob, float inv_t, T* grad,
-                                                                long long grad_stride, int vocab, int parts) {
-  constexpr int E = Vec<T>::kElements, kPart = kBackThreads * kBackVectors;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) backward_kernel(const T* logits, long long row_stride,
+                                                           const long long* __restrict__ ids, const float2* __restrict__ stats,
+                                                           const float* __restrict__ grad_logprob, float inv_t, T* grad,
+                                                           long long grad_stride, int vocab, int parts) {
+  constexpr int E = Vec<T>::kElements, kPart = THREADS * kBackVectors;
   const long long row = blockIdx.x / parts, t = ids[row];
   const int part = blockIdx.x - row * parts;
   const T* x = logits + row * row_stride;
@@ -477,7 +476,7 @@ __global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits,
   const bool last = part == parts - 1;
   if (t < 0 || t >= vocab) {
     clear(g, part == 0 ? 0 : min(vocab, cut.head + part * kPart * E), last ? vocab : min(vocab, cut.head + (part + 1) * kPart * E),
-          threadIdx.x, kBackThreads);
+          threadIdx.x, THREADS);
     return;
   }
   const uint4* p = reinterpret_cast<const uint4*>(x + cut.head);
@@ -485,7 +484,7 @@ __global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits,
   uint4 q[kBackVectors];
 #pragma unroll
   for (int j = 0; j < kBackVectors; ++j)
-    if (first + j * kBackThreads < end) q[j] = __ldcs(p + first + j * kBackThreads);
+    if (first + j * THREADS < end) q[j] = __ldcs(p + first + j * THREADS);
   const float c = inv_t * kLog2e, w = grad_logprob[row] * inv_t;
   const float2 st = stats[row];
   const pair_t cc = pair(c, c), less = pair(-st.y, -st.y), scale = pair(-w, -w);
@@ -495,7 +494,7 @@ __global__ void __launch_bounds__(kBackThreads) backward_kernel(const T* logits,
   const bool inside = at >= 0 && holder < cut.vectors;
 #pragma unroll
   for (int j = 0; j < kBackVectors; ++j) {
-    const int v = first + j * kBackThreads;
+    const int v = first + j * THREADS;
     if (v < end) {
       const bool own = inside && v == holder;
       const float xt = own ? load1(x + t) : 0.f;   // before it may be overwritten
@@ -618,6 +617,21 @@ int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, cons
   return launch(row_grad_kernel<T, 256, 8, kResident / 256>, 8);
 }
 
+// Small blocks where a row would leave most of a large one idle (16384 x 500 bf16: 29 us with 256 threads, 13 with 64).
+template <typename T>
+int launch_backward(const char* who, const void* logits, int64_t row_stride, const int64_t* ids, const float* stats,
+                    const float* grad_logprob, float temperature, void* grad, int64_t grad_stride, int64_t rows, int64_t vocab,
+                    cudaStream_t s) {
+  const int threads = vocab / Vec<T>::kElements <= 64 * kBackVectors ? 64 : 256;
+  const int64_t part = (int64_t)threads * kBackVectors * Vec<T>::kElements, parts = (vocab + part - 1) / part;
+  MOLT_REQUIRE(rows * parts < (1LL << 31), MOLT_E_CAPABILITY, "%s: more than 2^31 blocks of logits", who);
+  const auto kernel = threads == 64 ? backward_kernel<T, 64> : backward_kernel<T, 256>;
+  kernel<<<(unsigned)(rows * parts), threads, 0, s>>>(
+      reinterpret_cast<const T*>(logits), row_stride, reinterpret_cast<const long long*>(ids), reinterpret_cast<const float2*>(stats),
+      grad_logprob, 1.f / temperature, reinterpret_cast<T*>(grad), grad_stride, (int)vocab, (int)parts);
+  return launch_status("token_logprob backward_kernel");
+}
+
 }  // namespace
 }  // namespace molt
 
@@ -661,20 +675,8 @@ extern "C" int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row
   MOLT_REQUIRE(stats && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   MOLT_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, MOLT_E_VALUE, "%s: stats must be 8-byte aligned", who);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto* id = reinterpret_cast<const long long*>(token_ids);
-  auto* st = reinterpret_cast<const float2*>(stats);
-  const int64_t per_part = (int64_t)kBackThreads * kBackVectors * (dtype == MOLT_DTYPE_BF16 ? 8 : 4);
-  const int64_t parts = (vocab + per_part - 1) / per_part;
-  MOLT_REQUIRE(rows * parts < (1LL << 31), MOLT_E_CAPABILITY, "%s: more than 2^31 blocks of logits", who);
-  const unsigned blocks = (unsigned)(rows * parts);
-  if (dtype == MOLT_DTYPE_BF16)
-    backward_kernel<__nv_bfloat16><<<blocks, kBackThreads, 0, s>>>(
-        reinterpret_cast<const __nv_bfloat16*>(logits), row_stride, id, st, grad_logprob, 1.f / temperature,
-        reinterpret_cast<__nv_bfloat16*>(grad_logits), grad_stride, (int)vocab, (int)parts);
-  else
-    backward_kernel<float><<<blocks, kBackThreads, 0, s>>>(reinterpret_cast<const float*>(logits), row_stride, id, st,
-                                                           grad_logprob, 1.f / temperature,
-                                                           reinterpret_cast<float*>(grad_logits), grad_stride, (int)vocab,
-                                                           (int)parts);
-  return launch_status("token_logprob backward_kernel");
+  return dtype == MOLT_DTYPE_BF16 ? launch_backward<__nv_bfloat16>(who, logits, row_stride, token_ids, stats, grad_logprob, temperature,
+                                                                   grad_logits, grad_stride, rows, vocab, s)
+                                  : launch_backward<float>(who, logits, row_stride, token_ids, stats, grad_logprob, temperature,
+                                                           grad_logits, grad_stride, rows, vocab, s);
 }

@@ -89,7 +89,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, temperature: f
 def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weight: Optional[torch.Tensor] = None,
                              temperature: float = 1.0, out: Optional[torch.Tensor] = None
                              ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``(logprobs, grad)`` in one pass over the logits: the log-probabilities of :func:`token_logprobs` and
+    """``(logprobs, grad)`` in one pass over the logits: the log-probabilities of :func:`token_logprobs` (to rounding) and
     ``grad[..., v] = weight * d logprob / d logits[..., v]`` (``weight`` None: 1), rounded once to the logits' type.
 
     For callers that differentiate by hand, such as a head whose logits are not kept: ``out`` receives the gradient and may
