@@ -569,7 +569,9 @@ class QLoRAStep:
             if t is not None:
                 held.copy_(t)
 
-    def run(self, *inputs: Optional[torch.Tensor]) -> torch.Tensor:
+    def run(self, tokens: torch.Tensor, targets: torch.Tensor, *more: Optional[torch.Tensor]) -> torch.Tensor:
+        """One step; ``more`` is what the objective takes behind the targets."""
+        inputs = (tokens, targets, *more)
         if self.guard is not None:
             self.guard.check(self.steps)     # host-side: every peer is alive and about to run the same step
         if self.cuda_graph and self._graph is None and self._eager_steps >= 2:

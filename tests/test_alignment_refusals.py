@@ -216,3 +216,28 @@ def test_step_driver_arguments_are_checked_on_the_host():
             frozen_head_logprobs(*bad)
     with pytest.raises(CapabilityError):
         frozen_head_logprobs(hidden, head, ids)
+
+
+class _HostStep:
+    """A step driver without a device: model, optimizer and graph are stand-ins that record what they are given."""
+
+    def __new__(cls):
+        from molt_b200.qlora_step import CrossEntropy, QLoRAStep
+
+        class Optimizer:
+            def step(self, grad_scale, max_norm):
+                return None
+
+        step = object.__new__(QLoRAStep)
+        step.guard = step.shadows = step.max_grad_norm = step._graph = None
+        step.cuda_graph, step._eager_steps, step.steps, step.status_interval, step.world = False, 0, 0, 0, 1
+        step.objective, step.optimizer = CrossEntropy(), Optimizer()
+        step._forward_backward = lambda *inputs: inputs
+        return step
+
+
+def test_step_takes_tokens_and_targets_by_name():
+    step = _HostStep()
+    assert step.run(tokens=1, targets=2) == (1, 2)
+    assert step.run(1, targets=2) == (1, 2)
+    assert step.run(1, 2, 3, None) == (1, 2, 3, None)
