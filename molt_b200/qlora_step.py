@@ -553,7 +553,7 @@ class QLoRAStep:
     def _capture(self, *inputs) -> None:
         """Record forward + backward (+ the overlapped collectives) of one micro-batch once; every later step replays
         the recording (the kernels take raw pointers and never allocate or synchronise, so they are capture-safe)."""
-        self._static_inputs = tuple(None if t is None else t.clone() for t in inputs)
+        self._hold(*inputs)
         self._graph = torch.cuda.CUDAGraph()
         lib = _native.library()
         before = lib.molt_launch_count()
@@ -561,13 +561,16 @@ class QLoRAStep:
             self._static_loss = self._forward_backward(*self._static_inputs)
         self.graph_launches = int(lib.molt_launch_count() - before)   # library kernels recorded; each replay runs them
 
+    def _hold(self, *inputs) -> None:
+        self._static_inputs = tuple(None if t is None else t.detach().clone() for t in inputs)
+
     def _stage(self, *inputs) -> None:
         shapes = [None if t is None else t.shape for t in inputs]
         if shapes != [None if held is None else held.shape for held in self._static_inputs]:
             raise ValueError("the inputs of a captured step keep their number and shapes")
         for t, held in zip(inputs, self._static_inputs):
             if t is not None:
-                held.copy_(t)
+                held.copy_(t.detach())
 
     def run(self, tokens: torch.Tensor, targets: torch.Tensor, *more: Optional[torch.Tensor]) -> torch.Tensor:
         """One step; ``more`` is what the objective takes behind the targets."""

@@ -241,3 +241,14 @@ def test_step_takes_tokens_and_targets_by_name():
     assert step.run(tokens=1, targets=2) == (1, 2)
     assert step.run(1, targets=2) == (1, 2)
     assert step.run(1, 2, 3, None) == (1, 2, 3, None)
+
+
+def test_captured_step_keeps_no_graph_of_its_inputs():
+    """Log-probabilities handed over with their graph: the held copies must not take part in it."""
+    step = _HostStep()
+    weight = torch.nn.Parameter(torch.ones(3))
+    step._hold(torch.zeros(3, dtype=torch.int64), weight * 2, None)
+    step._stage(torch.ones(3, dtype=torch.int64), weight * 3, None)
+    tokens, old, mask = step._static_inputs
+    assert tokens.tolist() == [1, 1, 1] and old.tolist() == [3, 3, 3] and mask is None
+    assert old.grad_fn is None and not old.requires_grad
