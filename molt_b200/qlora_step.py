@@ -12,6 +12,7 @@ layers is still running (``molt_b200.data_parallel``).
 from __future__ import annotations
 
 import math
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import Optional
 
@@ -491,6 +492,30 @@ def attach_lora_shadows(model: nn.Module) -> list:
     return made
 
 
+@contextmanager
+def leaves_of_its_own(model: nn.Module):
+    """Stand-ins for ``model``'s trainable parameters: the same memory, gradients and attributes, but other autograd leaves.
+    All graphs of a leaf share its accumulation node and the stream that the node was made on, so a backward pass that is
+    recorded while an eager graph of the same leaves is alive would reach out of the recording to that stream, which
+    ends the process.  A graph of stand-ins shares no node with one made before."""
+    held, stand_ins = [], {}
+    for module in model.modules():
+        for name, p in module._parameters.items():
+            if p is not None and p.requires_grad:
+                held.append((module, name, p))
+    try:
+        for module, name, p in held:
+            if p not in stand_ins:
+                other = stand_ins[p] = nn.Parameter(p.detach())
+                other.grad = p.grad
+                vars(other).update(vars(p))
+            module._parameters[name] = stand_ins[p]
+        yield
+    finally:
+        for module, name, p in held:
+            module._parameters[name] = p
+
+
 class QLoRAStep:
     """Holds model, gradient arena and optimiser; ``run(tokens, targets)`` is one data-parallel training step on the
     cross-entropy, or with another ``objective`` (:class:`PolicyObjective`, :class:`PreferenceObjective`) ``run`` takes that
@@ -557,7 +582,7 @@ class QLoRAStep:
         self._graph = torch.cuda.CUDAGraph()
         lib = _native.library()
         before = lib.molt_launch_count()
-        with torch.cuda.graph(self._graph):
+        with leaves_of_its_own(self.model), torch.cuda.graph(self._graph):
             self._static_loss = self._forward_backward(*self._static_inputs)
         self.graph_launches = int(lib.molt_launch_count() - before)   # library kernels recorded; each replay runs them
 

@@ -252,3 +252,44 @@ def test_captured_step_keeps_no_graph_of_its_inputs():
     tokens, old, mask = step._static_inputs
     assert tokens.tolist() == [1, 1, 1] and old.tolist() == [3, 3, 3] and mask is None
     assert old.grad_fn is None and not old.requires_grad
+
+
+def _graph_nodes(tensor):
+    seen, todo = set(), [tensor.grad_fn]
+    while todo:
+        node = todo.pop()
+        if node is not None and node not in seen:
+            seen.add(node)
+            todo += [following for following, _ in node.next_functions]
+    return seen
+
+
+def test_recording_shares_no_node_with_an_eager_graph():
+    """A graph that the caller keeps (log-probabilities not detached, say) shares its leaves' accumulation nodes, and the
+    stream they were made on, with every later graph of the same leaves; a recording has leaves of its own."""
+    from molt_b200.data_parallel import GradArena
+    from molt_b200.qlora_step import leaves_of_its_own
+
+    model = torch.nn.Sequential(torch.nn.Linear(3, 4), torch.nn.Linear(4, 2))
+    model[1].weight.requires_grad_(False)
+    model[1].bias = model[1].bias
+    arena = GradArena(model.parameters())
+    before = list(model.parameters())
+    x = torch.randn(5, 3)
+    kept = model(x).square().sum()
+    with leaves_of_its_own(model):
+        inside = list(model.parameters())
+        assert all(a.data_ptr() == b.data_ptr() and a.requires_grad == b.requires_grad for a, b in zip(inside, before))
+        assert all(vars(a) == vars(b) and (a is not b) == b.requires_grad for a, b in zip(inside, before))
+        loss = model(x).square().sum()
+        assert not _graph_nodes(loss) & _graph_nodes(kept)
+        loss.backward()
+    got = arena.flat.clone()
+    assert all(a is b for a, b in zip(model.parameters(), before))
+    arena.zero()
+    kept.backward()
+    assert bool(got.any()) and torch.equal(got, arena.flat)
+    with pytest.raises(KeyError):
+        with leaves_of_its_own(model):
+            raise KeyError
+    assert all(a is b for a, b in zip(model.parameters(), before))

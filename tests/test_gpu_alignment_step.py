@@ -243,3 +243,24 @@ def test_policy_step_in_the_static_microbatch_runner(native_library):
     eager = build(x, ids, old, adv)
     eager.backward()
     assert torch.equal(loss, eager.detach()) and torch.equal(grad, weight.grad)
+
+
+def test_step_captured_while_the_caller_keeps_graphs_of_the_model(native_library):
+    """Old log-probabilities taken from the model itself and handed over with their graph, before and after the capture."""
+    from molt_b200.qlora_step import QLoRAStep
+
+    shape = _shape()
+    runs = []
+    for graph in (False, True):
+        step = QLoRAStep(shape, torch.device("cuda"), lr=5e-3, objective=_objective("policy"), max_grad_norm=0.5, cuda_graph=graph)
+        losses, kept = [], []
+        for i in range(5):
+            tokens, targets, _, advantages, mask, ref = _batch(shape, "policy", i)
+            kept.append(step.model.logprobs(tokens, targets))
+            assert kept[-1].requires_grad
+            losses.append(step.run(tokens, targets, kept[-1], advantages, mask, ref).clone())
+        assert (step.replayed_launches > 0) == graph
+        assert all(t is None or t.grad_fn is None for t in step._static_inputs)
+        runs.append((torch.stack(losses), step.optimizer.flat.clone()))
+    for a, b in zip(*runs):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
