@@ -22,6 +22,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from molt_b200 import _native
+from molt_b200.core.errors import CapabilityError
 from molt_b200.data_parallel import GradArena, ParamArena, StepGuard, lora_parameters
 from molt_b200.kernels.policy_loss import clipped_policy_loss, preference_loss
 from molt_b200.kernels.token_logprobs import token_logprobs, token_logprobs_with_grad
@@ -345,7 +346,8 @@ class _FrozenHeadLogprobs(torch.autograd.Function):
     def forward(ctx, hidden, head, token_ids, chunk, temperature, trained):
         hidden = hidden.contiguous()
         rows, vocab = hidden.shape[0], head.shape[0]
-        native = hidden.dtype == torch.bfloat16 and head.dtype == torch.bfloat16 and vocab % 64 == 0 and hidden.shape[1] % 64 == 0
+        native = (hidden.dtype == torch.bfloat16 and head.dtype == torch.bfloat16 and vocab % 64 == 0 and hidden.shape[1] % 64 == 0
+                  and head.is_contiguous() and (head.data_ptr() | hidden.data_ptr()) % 16 == 0)
         logprobs = torch.empty(rows, dtype=torch.float32, device=hidden.device)
         unit = torch.empty_like(hidden) if trained else None
         for start in range(0, rows, chunk):
@@ -377,6 +379,10 @@ def frozen_head_logprobs(hidden: torch.Tensor, head: torch.Tensor, token_ids: to
         raise ValueError("the head must be frozen")
     if hidden.dim() != 2 or head.dim() != 2 or hidden.shape[1] != head.shape[1] or token_ids.shape != hidden.shape[:1]:
         raise ValueError("hidden must be [rows, width], head [vocab, width] and token_ids [rows]")
+    if head.device != hidden.device or token_ids.device != hidden.device:
+        raise ValueError("hidden, head and token_ids must be on one device")
+    if hidden.device.type != "cuda":
+        raise CapabilityError("frozen_head_logprobs requires CUDA tensors")
     if chunk < 1:
         raise ValueError("chunk must be positive")
     trained = hidden.requires_grad and torch.is_grad_enabled()

@@ -293,3 +293,15 @@ def test_recording_shares_no_node_with_an_eager_graph():
         with leaves_of_its_own(model):
             raise KeyError
     assert all(a is b for a, b in zip(model.parameters(), before))
+
+
+def test_frozen_head_logprobs_needs_one_cuda_device():
+    """Sizes that the GEMM kernel takes: a host pointer must not reach it."""
+    from molt_b200.qlora_step import frozen_head_logprobs
+
+    hidden, head, ids = torch.zeros(4, 64).bfloat16(), torch.zeros(128, 64).bfloat16(), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(CapabilityError):
+        frozen_head_logprobs(hidden, head, ids)
+    for bad in ((hidden, head.to("meta"), ids), (hidden.to("meta"), head, ids.to("meta")), (hidden, head, ids.to("meta"))):
+        with pytest.raises(ValueError):
+            frozen_head_logprobs(*bad)

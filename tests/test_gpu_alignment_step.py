@@ -264,3 +264,34 @@ def test_step_captured_while_the_caller_keeps_graphs_of_the_model(native_library
         runs.append((torch.stack(losses), step.optimizer.flat.clone()))
     for a, b in zip(*runs):
         assert bool(a.isfinite().all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("form", ["transposed", "columns", "offset head", "offset hidden"])
+def test_frozen_head_logprobs_of_a_head_that_is_no_dense_matrix(native_library, form):
+    """Strides and offsets that the head's GEMM kernel does not take; bounds as for the dense head, on the plain product's logits."""
+    from molt_b200.qlora_step import frozen_head_logprobs
+
+    gen = _gen(31)
+    rows, width, vocab = 9, 64, 128
+    hidden = torch.randn(rows * width + 1, device="cuda", generator=gen).bfloat16()
+    hidden = hidden[form == "offset hidden":][:rows * width].view(rows, width).requires_grad_()
+    dense = (torch.randn(vocab, width, device="cuda", generator=gen) * 0.2).bfloat16()
+    if form == "transposed":
+        head = dense.t().contiguous().t()
+    elif form == "columns":
+        head = torch.cat([dense, dense], 1)[:, width:]
+    elif form == "offset head":
+        head = torch.cat([dense.new_zeros(1), dense.flatten()])[1:].view(vocab, width)
+    else:
+        head = dense
+    assert torch.equal(head, dense)
+    ids = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+    logits = (hidden.detach() @ head.t()).double()
+    lsm = torch.log_softmax(logits, -1)
+    want = lsm.gather(1, ids[:, None])[:, 0]
+    lp = frozen_head_logprobs(hidden, head, ids)
+    _close(lp.detach(), want, 2.0 ** -24 * (200 + 8 * want.abs()))
+    (grad,) = torch.autograd.grad(lp.sum(), hidden)
+    row = torch.zeros_like(lsm).scatter_(1, ids[:, None], 1.0) - lsm.exp()
+    exact = row @ dense.double()
+    _close(grad, exact, (row.abs() @ dense.double().abs() * (HALF_BF16 + 2 ** -12) + exact.abs() * 2.1 * HALF_BF16) * 1.01 + 1e-30)
