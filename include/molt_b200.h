@@ -318,26 +318,29 @@ int molt_mlp_bwd_t(const molt_lora_proj* gate, const molt_lora_proj* up, const m
  * The reference trains on next-token cross-entropy alone; these entry points have no counterpart there. */
 
 /* Log-probability of one given token per row of logits [rows, vocab] (dtype MOLT_DTYPE_BF16 or MOLT_DTYPE_F32; row r begins
- * row_stride * r elements behind the first, row_stride 0 reads one row for all):
+ * group_stride * (r / group_rows) + row_stride * (r % group_rows) elements behind the first, or row_stride * r with group_rows 0;
+ * a stride of 0 repeats rows):
  *   logprob[r] = (x[t] - max) / T - ln(sum_v exp((x[v] - max) / T)),   t = token_ids[r], T = temperature,
  * 1e-30 <= T <= 1e30.
  * A token id outside [0, vocab) (an ignore index such as -100) gives 0 and its row is not read.  Logits of -inf have
  * probability zero; a row without a finite logit, or with NaN or +inf, gives NaN.  stats (optional): [rows, 2] floats, 8-byte aligned,
  * for molt_token_logprob_bwd (what the exponents were taken from, and log2 of the sum).  fp32 arithmetic. */
-int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, float temperature,
-                           float* logprob, float* stats, int64_t rows, int64_t vocab, uintptr_t stream);
+int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, int64_t group_rows, int64_t group_stride,
+                           const int64_t* token_ids, float temperature, float* logprob, float* stats, int64_t rows, int64_t vocab,
+                           uintptr_t stream);
 
 /* grad_logits[r, v] = grad_logprob[r] * (1[v == t] - softmax(x / T)[v]) / T, rounded once; rows whose token id is outside
  * [0, vocab) get zeros.  grad_logits has the logits' dtype and its own row stride (>= vocab); it may be the logits
- * themselves (same address and stride) and must not overlap them otherwise. */
-int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, const float* stats,
-                           const float* grad_logprob, float temperature, void* grad_logits, int64_t grad_stride,
-                           int64_t rows, int64_t vocab, uintptr_t stream);
+ * themselves (same address and stride, one group) and must not overlap them otherwise. */
+int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, int64_t group_rows, int64_t group_stride,
+                           const int64_t* token_ids, const float* stats, const float* grad_logprob, float temperature,
+                           void* grad_logits, int64_t grad_stride, int64_t rows, int64_t vocab, uintptr_t stream);
 
 /* Both in one pass over the logits: logprob as molt_token_logprob_fwd (to rounding: it adds in another order), grad_logits as molt_token_logprob_bwd with
  * grad_logprob[r] = weight[r] (weight NULL: 1).  Meant for a loss whose gradient scales rows: with weight 1 the caller
  * multiplies by dLoss/dlogprob[r] behind the head's second GEMM, where a row is the hidden width and not the vocabulary. */
-int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids, const float* weight,
+int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, int64_t group_rows, int64_t group_stride,
+                           const int64_t* token_ids, const float* weight,
                             float temperature, float* logprob, void* grad_logits, int64_t grad_stride, int64_t rows,
                             int64_t vocab, uintptr_t stream);
 

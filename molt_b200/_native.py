@@ -179,11 +179,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.molt_mlp_bwd_t.argtypes = [proj, proj, proj, vp, vp, vp, vp, vp, vp, ctypes.POINTER(vp), i32, i64, vp, sz, up]
     f64, pi64 = ctypes.c_double, ctypes.POINTER(ctypes.c_int64)
     lib.molt_token_logprob_fwd.restype = i32
-    lib.molt_token_logprob_fwd.argtypes = [vp, i32, i64, vp, f32, vp, vp, i64, i64, up]
+    lib.molt_token_logprob_fwd.argtypes = [vp, i32, i64, i64, i64, vp, f32, vp, vp, i64, i64, up]
     lib.molt_token_logprob_bwd.restype = i32
-    lib.molt_token_logprob_bwd.argtypes = [vp, i32, i64, vp, vp, vp, f32, vp, i64, i64, i64, up]
+    lib.molt_token_logprob_bwd.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, f32, vp, i64, i64, i64, up]
     lib.molt_token_logprob_grad.restype = i32
-    lib.molt_token_logprob_grad.argtypes = [vp, i32, i64, vp, vp, f32, vp, vp, i64, i64, i64, up]
+    lib.molt_token_logprob_grad.argtypes = [vp, i32, i64, i64, i64, vp, vp, f32, vp, vp, i64, i64, i64, up]
     lib.molt_policy_loss_workspace_bytes.restype = sz
     lib.molt_policy_loss_workspace_bytes.argtypes = [i64, i64]
     lib.molt_policy_loss_fwd.restype = i32

@@ -215,6 +215,18 @@ __device__ __forceinline__ void row_join(float& m, float& s, float c, unsigned r
   }
 }
 
+// Where the rows of logits lie: `group` rows (0: all of them) one `stride` apart, then the next group.  Two strides are what
+// logits[:, :-1] needs to be read where it is; the division is one per block.
+struct Layout {
+  long long stride, group_stride;
+  unsigned group;
+  __device__ __forceinline__ long long of(unsigned row) const {
+    if (group == 0) return row * stride;
+    const unsigned g = row / group;
+    return g * group_stride + (row - g * group) * stride;
+  }
+};
+
 // Where a row's 16-byte vectors begin and how many there are; `head` elements stand in front of them, `tail` behind.
 template <typename T>
 struct Cut {
@@ -265,11 +277,11 @@ __device__ __forceinline__ bool cut_alike(const T* a, const T* b) {
 // long 256 threads were 2-4 % slower than 512, and 8 vectors in flight 10 %.
 template <typename T, int THREADS, int NB, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
-    row_kernel(const T* __restrict__ logits, long long row_stride, const long long* __restrict__ ids, float inv_t,
+    row_kernel(const T* __restrict__ logits, Layout layout, const long long* __restrict__ ids, float inv_t,
                float* __restrict__ logprob, float2* __restrict__ stats, int vocab) {
   const unsigned size = cluster_size(), rank = cluster_rank();
   const long long row = blockIdx.x / size, t = ids[row];
-  const T* x = logits + row * row_stride;
+  const T* x = logits + layout.of((unsigned)row);
   const int first = rank * THREADS + threadIdx.x, step = size * THREADS;
   if (t < 0 || t >= vocab) {
     if (first == 0) {
@@ -333,13 +345,13 @@ constexpr int kRing = 5, kRingBatch = 2;
 
 template <typename T, int THREADS, int CLUSTER, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
-    row_grad_kernel(const T* logits, long long row_stride, const long long* __restrict__ ids, const float* __restrict__ weight,
+    row_grad_kernel(const T* logits, Layout layout, const long long* __restrict__ ids, const float* __restrict__ weight,
                     float inv_t, float* __restrict__ logprob, T* grad, long long grad_stride, int vocab) {
   constexpr int E = Vec<T>::kElements, B = kRingBatch, R = kRing, kStep = CLUSTER * THREADS, kBatch = B * kStep;
   extern __shared__ uint4 ring[];   // [R * B][THREADS]
   const unsigned rank = CLUSTER > 1 ? cluster_rank() : 0;
   const long long row = blockIdx.x / CLUSTER, t = ids[row];
-  const T* x = logits + row * row_stride;
+  const T* x = logits + layout.of((unsigned)row);
   T* g = grad + row * grad_stride;
   const int first = rank * THREADS + threadIdx.x;
   if (t < 0 || t >= vocab) {
@@ -463,14 +475,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 constexpr int kBackVectors = 4;
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) backward_kernel(const T* logits, long long row_stride,
+__global__ void __launch_bounds__(THREADS) backward_kernel(const T* logits, Layout layout,
                                                            const long long* __restrict__ ids, const float2* __restrict__ stats,
                                                            const float* __restrict__ grad_logprob, float inv_t, T* grad,
                                                            long long grad_stride, int vocab, int parts) {
   constexpr int E = Vec<T>::kElements, kPart = THREADS * kBackVectors;
   const long long row = blockIdx.x / parts, t = ids[row];
   const int part = blockIdx.x - row * parts;
-  const T* x = logits + row * row_stride;
+  const T* x = logits + layout.of((unsigned)row);
   T* g = grad + row * grad_stride;
   const Cut<T> cut(x, vocab);
   const bool last = part == parts - 1;
@@ -511,8 +523,8 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const T* logits, long
   }
 }
 
-int check_rows(const char* who, const void* logits, int dtype, int64_t row_stride, const int64_t* ids, float temperature,
-               int64_t rows, int64_t vocab) {
+int check_rows(const char* who, const void* logits, int dtype, int64_t row_stride, int64_t group_rows, int64_t group_stride,
+               const int64_t* ids, float temperature, int64_t rows, int64_t vocab) {
   MOLT_REQUIRE(rows >= 0 && vocab > 0, MOLT_E_VALUE, "%s: bad shape", who);
   MOLT_REQUIRE(rows <= (1LL << 27) && vocab <= (1LL << 30), MOLT_E_CAPABILITY, "%s: more than 2^27 rows or 2^30 columns", who);
   MOLT_REQUIRE(dtype == MOLT_DTYPE_BF16 || dtype == MOLT_DTYPE_F32, MOLT_E_CAPABILITY, "%s: logits must be bf16 or fp32", who);
@@ -522,28 +534,39 @@ int check_rows(const char* who, const void* logits, int dtype, int64_t row_strid
   MOLT_REQUIRE(logits && ids, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   MOLT_REQUIRE(reinterpret_cast<uintptr_t>(ids) % 8 == 0, MOLT_E_VALUE, "%s: token_ids are not aligned to their type", who);
   MOLT_REQUIRE(row_stride == 0 || row_stride >= vocab, MOLT_E_VALUE, "%s: rows of logits overlap", who);
+  MOLT_REQUIRE(group_rows >= 0, MOLT_E_VALUE, "%s: bad group_rows", who);
+  MOLT_REQUIRE(group_rows == 0 || group_stride == 0 || group_stride >= vocab, MOLT_E_VALUE, "%s: groups of logits overlap", who);
   MOLT_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == MOLT_DTYPE_BF16 ? 2 : 4) == 0, MOLT_E_VALUE,
                "%s: logits are not aligned to their type", who);
   return MOLT_OK;
 }
 
 // The gradient may lie over the logits exactly, or beside them (also in other columns of the same wider rows).
-int check_grad(const char* who, const void* logits, int dtype, int64_t row_stride, const void* grad, int64_t grad_stride,
-               int64_t rows, int64_t vocab) {
+int check_grad(const char* who, const void* logits, int dtype, const Layout& layout, const void* grad, int64_t grad_stride, int64_t rows,
+               int64_t vocab) {
   if (rows == 0) return MOLT_OK;
   const int64_t size = dtype == MOLT_DTYPE_BF16 ? 2 : 4;
   MOLT_REQUIRE(grad != nullptr, MOLT_E_VALUE, "%s: NULL gradient pointer", who);
   MOLT_REQUIRE(reinterpret_cast<uintptr_t>(grad) % size == 0, MOLT_E_VALUE, "%s: the gradient is not aligned to its type", who);
   MOLT_REQUIRE(grad_stride >= vocab, MOLT_E_VALUE, "%s: rows of the gradient overlap", who);
   const intptr_t a = reinterpret_cast<intptr_t>(logits), b = reinterpret_cast<intptr_t>(grad);
-  if (a == b && (row_stride == grad_stride || rows == 1)) return MOLT_OK;
-  const intptr_t a_end = a + ((rows - 1) * row_stride + vocab) * size, b_end = b + ((rows - 1) * grad_stride + vocab) * size;
+  const bool alike = layout.group == 0 && layout.stride == grad_stride;
+  if (a == b && (alike || rows == 1)) return MOLT_OK;
+  const int64_t groups = layout.group == 0 ? 1 : (rows - 1) / layout.group + 1, in_group = layout.group == 0 ? rows : layout.group;
+  const intptr_t a_end = a + ((groups - 1) * layout.group_stride + (in_group - 1) * layout.stride + vocab) * size;
+  const intptr_t b_end = b + ((rows - 1) * grad_stride + vocab) * size;
   if (a_end <= b || b_end <= a) return MOLT_OK;
-  if (row_stride == grad_stride) {
-    const intptr_t pitch = row_stride * size, shift = (((b - a) % pitch) + pitch) % pitch;
+  if (alike) {
+    const intptr_t pitch = grad_stride * size, shift = (((b - a) % pitch) + pitch) % pitch;
     if (shift >= vocab * size && shift <= pitch - vocab * size) return MOLT_OK;
   }
   return fail(MOLT_E_VALUE, "%s: the gradient overlaps the logits without being the same rows", who);
+}
+
+// Rows of one group, or of groups that follow each other like their rows, need no division.
+Layout layout_of(int64_t row_stride, int64_t group_rows, int64_t group_stride, int64_t rows) {
+  const bool one = group_rows == 0 || group_rows >= rows || group_stride == group_rows * row_stride;
+  return {row_stride, one ? 0 : group_stride, one ? 0u : (unsigned)group_rows};
 }
 
 template <typename... Params, typename... Args>
@@ -579,13 +602,13 @@ int threads_for(int64_t rows, int64_t vectors, int most, int resident) {
 // * with gradient, until a thread has at most 20 vectors, so that the rows in flight stay in the L2;
 // * in both directions, as long as the rows alone do not fill the device and a thread keeps at least 4 vectors.
 template <typename T>
-int launch_forward(const void* logits, int64_t row_stride, const int64_t* ids, float temperature, float* logprob, float* stats,
+int launch_forward(const void* logits, const Layout& layout, const int64_t* ids, float temperature, float* logprob, float* stats,
                    int64_t rows, int64_t vocab, cudaStream_t s) {
   constexpr int kResident = sizeof(T) == 2 ? 2048 : 1536;   // threads per SM: 32 registers each, or 40
   const int64_t vectors = vocab / Vec<T>::kElements;
   const int threads = threads_for(rows, vectors, 512, kResident);
   const auto launch = [&](auto kernel, int cluster) {
-    return launch_clusters("token_logprob row_kernel", kernel, rows, cluster, threads, 0, s, reinterpret_cast<const T*>(logits), row_stride,
+    return launch_clusters("token_logprob row_kernel", kernel, rows, cluster, threads, 0, s, reinterpret_cast<const T*>(logits), layout,
                            reinterpret_cast<const long long*>(ids), 1.f / temperature, logprob, reinterpret_cast<float2*>(stats), vocab);
   };
   if (threads == 64) return launch(row_kernel<T, 64, 4, kResident / 64>, 1);
@@ -597,14 +620,14 @@ int launch_forward(const void* logits, int64_t row_stride, const int64_t* ids, f
 }
 
 template <typename T>
-int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, const float* weight, float temperature, float* logprob,
+int launch_grad(const void* logits, const Layout& layout, const int64_t* ids, const float* weight, float temperature, float* logprob,
                 void* grad, int64_t grad_stride, int64_t rows, int64_t vocab, cudaStream_t s) {
   constexpr int kResident = 1280;   // threads per SM: 48 registers and 160 bytes of the ring each
   const int64_t vectors = vocab / Vec<T>::kElements;
   const int threads = threads_for(rows, vectors, 256, kResident);
   const auto launch = [&](auto kernel, int cluster) {
     return launch_clusters("token_logprob row_grad_kernel", kernel, rows, cluster, threads, threads * kRing * kRingBatch * sizeof(uint4), s,
-                           reinterpret_cast<const T*>(logits), row_stride, reinterpret_cast<const long long*>(ids), weight,
+                           reinterpret_cast<const T*>(logits), layout, reinterpret_cast<const long long*>(ids), weight,
                            1.f / temperature, logprob, reinterpret_cast<T*>(grad), grad_stride, vocab);
   };
   if (threads == 64) return launch(row_grad_kernel<T, 64, 1, kResident / 64>, 1);
@@ -619,7 +642,7 @@ int launch_grad(const void* logits, int64_t row_stride, const int64_t* ids, cons
 
 // Small blocks where a row would leave most of a large one idle (16384 x 500 bf16: 29 us with 256 threads, 13 with 64).
 template <typename T>
-int launch_backward(const char* who, const void* logits, int64_t row_stride, const int64_t* ids, const float* stats,
+int launch_backward(const char* who, const void* logits, const Layout& layout, const int64_t* ids, const float* stats,
                     const float* grad_logprob, float temperature, void* grad, int64_t grad_stride, int64_t rows, int64_t vocab,
                     cudaStream_t s) {
   const int threads = vocab / Vec<T>::kElements <= 64 * kBackVectors ? 64 : 256;
@@ -627,7 +650,7 @@ int launch_backward(const char* who, const void* logits, int64_t row_stride, con
   MOLT_REQUIRE(rows * parts < (1LL << 31), MOLT_E_CAPABILITY, "%s: more than 2^31 blocks of logits", who);
   const auto kernel = threads == 64 ? backward_kernel<T, 64> : backward_kernel<T, 256>;
   kernel<<<(unsigned)(rows * parts), threads, 0, s>>>(
-      reinterpret_cast<const T*>(logits), row_stride, reinterpret_cast<const long long*>(ids), reinterpret_cast<const float2*>(stats),
+      reinterpret_cast<const T*>(logits), layout, reinterpret_cast<const long long*>(ids), reinterpret_cast<const float2*>(stats),
       grad_logprob, 1.f / temperature, reinterpret_cast<T*>(grad), grad_stride, (int)vocab, (int)parts);
   return launch_status("token_logprob backward_kernel");
 }
@@ -637,46 +660,52 @@ int launch_backward(const char* who, const void* logits, int64_t row_stride, con
 
 using namespace molt;
 
-extern "C" int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids,
-                                      float temperature, float* logprob, float* stats, int64_t rows, int64_t vocab,
-                                      uintptr_t stream) {
-  if (int rc = check_rows("molt_token_logprob_fwd", logits, dtype, row_stride, token_ids, temperature, rows, vocab)) return rc;
+extern "C" int molt_token_logprob_fwd(const void* logits, int dtype, int64_t row_stride, int64_t group_rows,
+                                      int64_t group_stride, const int64_t* token_ids, float temperature, float* logprob,
+                                      float* stats, int64_t rows, int64_t vocab, uintptr_t stream) {
+  const char* who = "molt_token_logprob_fwd";
+  if (int rc = check_rows(who, logits, dtype, row_stride, group_rows, group_stride, token_ids, temperature, rows, vocab)) return rc;
   if (rows == 0) return MOLT_OK;
-  MOLT_REQUIRE(logprob != nullptr, MOLT_E_VALUE, "molt_token_logprob_fwd: NULL tensor pointer");
-  MOLT_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, MOLT_E_VALUE, "molt_token_logprob_fwd: stats must be 8-byte aligned");
+  MOLT_REQUIRE(logprob != nullptr, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
+  MOLT_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, MOLT_E_VALUE, "%s: stats must be 8-byte aligned", who);
+  const Layout layout = layout_of(row_stride, group_rows, group_stride, rows);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == MOLT_DTYPE_BF16
-             ? launch_forward<__nv_bfloat16>(logits, row_stride, token_ids, temperature, logprob, stats, rows, vocab, s)
-             : launch_forward<float>(logits, row_stride, token_ids, temperature, logprob, stats, rows, vocab, s);
+             ? launch_forward<__nv_bfloat16>(logits, layout, token_ids, temperature, logprob, stats, rows, vocab, s)
+             : launch_forward<float>(logits, layout, token_ids, temperature, logprob, stats, rows, vocab, s);
 }
 
-extern "C" int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids,
-                                       const float* weight, float temperature, float* logprob, void* grad_logits,
-                                       int64_t grad_stride, int64_t rows, int64_t vocab, uintptr_t stream) {
+extern "C" int molt_token_logprob_grad(const void* logits, int dtype, int64_t row_stride, int64_t group_rows,
+                                       int64_t group_stride, const int64_t* token_ids, const float* weight, float temperature,
+                                       float* logprob, void* grad_logits, int64_t grad_stride, int64_t rows, int64_t vocab,
+                                       uintptr_t stream) {
   const char* who = "molt_token_logprob_grad";
-  if (int rc = check_rows(who, logits, dtype, row_stride, token_ids, temperature, rows, vocab)) return rc;
-  if (int rc = check_grad(who, logits, dtype, row_stride, grad_logits, grad_stride, rows, vocab)) return rc;
+  if (int rc = check_rows(who, logits, dtype, row_stride, group_rows, group_stride, token_ids, temperature, rows, vocab)) return rc;
+  const Layout layout = layout_of(row_stride, group_rows, group_stride, rows);
+  if (int rc = check_grad(who, logits, dtype, layout, grad_logits, grad_stride, rows, vocab)) return rc;
   if (rows == 0) return MOLT_OK;
   MOLT_REQUIRE(logprob != nullptr, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == MOLT_DTYPE_BF16 ? launch_grad<__nv_bfloat16>(logits, row_stride, token_ids, weight, temperature, logprob, grad_logits,
+  return dtype == MOLT_DTYPE_BF16 ? launch_grad<__nv_bfloat16>(logits, layout, token_ids, weight, temperature, logprob, grad_logits,
                                                                grad_stride, rows, vocab, s)
-                                  : launch_grad<float>(logits, row_stride, token_ids, weight, temperature, logprob, grad_logits,
+                                  : launch_grad<float>(logits, layout, token_ids, weight, temperature, logprob, grad_logits,
                                                        grad_stride, rows, vocab, s);
 }
 
-extern "C" int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, const int64_t* token_ids,
-                                      const float* stats, const float* grad_logprob, float temperature, void* grad_logits,
-                                      int64_t grad_stride, int64_t rows, int64_t vocab, uintptr_t stream) {
+extern "C" int molt_token_logprob_bwd(const void* logits, int dtype, int64_t row_stride, int64_t group_rows,
+                                      int64_t group_stride, const int64_t* token_ids, const float* stats,
+                                      const float* grad_logprob, float temperature, void* grad_logits, int64_t grad_stride,
+                                      int64_t rows, int64_t vocab, uintptr_t stream) {
   const char* who = "molt_token_logprob_bwd";
-  if (int rc = check_rows(who, logits, dtype, row_stride, token_ids, temperature, rows, vocab)) return rc;
-  if (int rc = check_grad(who, logits, dtype, row_stride, grad_logits, grad_stride, rows, vocab)) return rc;
+  if (int rc = check_rows(who, logits, dtype, row_stride, group_rows, group_stride, token_ids, temperature, rows, vocab)) return rc;
+  const Layout layout = layout_of(row_stride, group_rows, group_stride, rows);
+  if (int rc = check_grad(who, logits, dtype, layout, grad_logits, grad_stride, rows, vocab)) return rc;
   if (rows == 0) return MOLT_OK;
   MOLT_REQUIRE(stats && grad_logprob, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   MOLT_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, MOLT_E_VALUE, "%s: stats must be 8-byte aligned", who);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == MOLT_DTYPE_BF16 ? launch_backward<__nv_bfloat16>(who, logits, row_stride, token_ids, stats, grad_logprob, temperature,
+  return dtype == MOLT_DTYPE_BF16 ? launch_backward<__nv_bfloat16>(who, logits, layout, token_ids, stats, grad_logprob, temperature,
                                                                    grad_logits, grad_stride, rows, vocab, s)
-                                  : launch_backward<float>(who, logits, row_stride, token_ids, stats, grad_logprob, temperature,
+                                  : launch_backward<float>(who, logits, layout, token_ids, stats, grad_logprob, temperature,
                                                            grad_logits, grad_stride, rows, vocab, s);
 }

@@ -25,27 +25,39 @@ def _check(logits: torch.Tensor, token_ids: torch.Tensor) -> int:
     return _DTYPES[logits.dtype]
 
 
-def _rows(logits: torch.Tensor) -> torch.Tensor:
-    """``[rows, vocab]`` with neighbouring columns: a view where the strides allow it, else a copy."""
-    if logits.dim() == 2 and logits.is_contiguous():
-        return logits
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    if (rows.shape[1] != 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and 0 < rows.stride(0) < rows.shape[1]):
-        rows = rows.contiguous()
-    return rows
+def _read_where_it_is(logits: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """The tensor, or a copy where it has to be one, and how its rows lie: (row stride, rows per group, group stride).  Rows that
+    two strides describe, such as those of ``logits[:, :-1]``, are read where they are."""
+    vocab = logits.shape[-1]
+    if logits.is_contiguous():
+        return logits, (vocab, 0, 0)
+    levels: list = []   # (extent, stride) of the leading dimensions from the last to the first, joined where they follow on
+    for extent, stride in zip(reversed(logits.shape[:-1]), reversed(logits.stride()[:-1])):
+        if extent == 1:
+            continue
+        if levels and stride == levels[-1][0] * levels[-1][1]:
+            levels[-1] = (levels[-1][0] * extent, levels[-1][1])
+        else:
+            levels.append((extent, stride))
+    if len(levels) > 2 or (vocab != 1 and logits.stride(-1) != 1) or any(0 < stride < vocab for _, stride in levels):
+        return logits.contiguous(), (vocab, 0, 0)
+    levels += [(0, vocab)] * (2 - len(levels))
+    (group_rows, row_stride), (_, group_stride) = levels
+    return logits, (row_stride, group_rows, group_stride)
 
 
 def _stride(rows: torch.Tensor) -> int:
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
-def _forward(rows: torch.Tensor, ids: torch.Tensor, temperature: float, stats: Optional[torch.Tensor]) -> torch.Tensor:
+def _forward(rows: torch.Tensor, layout: Tuple[int, int, int], ids: torch.Tensor, temperature: float,
+             stats: Optional[torch.Tensor]) -> torch.Tensor:
     device = rows.device
     logprobs = torch.empty(ids.shape, dtype=torch.float32, device=device)
     with _native.on_device(device):
         _native.check(_native.library().molt_token_logprob_fwd(
-            rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), temperature, logprobs.data_ptr(),
-            _native.ptr(stats), rows.shape[0], rows.shape[1], _native.stream_handle(device)))
+            rows.data_ptr(), _DTYPES[rows.dtype], *layout, ids.data_ptr(), temperature, logprobs.data_ptr(), _native.ptr(stats),
+            ids.numel(), rows.shape[-1], _native.stream_handle(device)))
     return logprobs
 
 
@@ -54,11 +66,11 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, token_ids: torch.Tensor, temperature: float) -> torch.Tensor:
-        rows, ids = _rows(logits), token_ids.contiguous()
-        stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=rows.device)
+        (rows, layout), ids = _read_where_it_is(logits), token_ids.contiguous()
+        stats = torch.empty((ids.numel(), 2), dtype=torch.float32, device=rows.device)
         ctx.save_for_backward(rows, ids, stats)
-        ctx.shape, ctx.temperature = logits.shape, temperature
-        return _forward(rows, ids, temperature, stats)
+        ctx.layout, ctx.temperature = layout, temperature
+        return _forward(rows, layout, ids, temperature, stats)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -68,22 +80,22 @@ class _TokenLogprobs(torch.autograd.Function):
         grad = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
         with _native.on_device(rows.device):
             _native.check(_native.library().molt_token_logprob_bwd(
-                rows.data_ptr(), _DTYPES[rows.dtype], _stride(rows), ids.data_ptr(), stats.data_ptr(), grad_output.data_ptr(),
-                ctx.temperature, grad.data_ptr(), grad.shape[1], rows.shape[0], rows.shape[1],
+                rows.data_ptr(), _DTYPES[rows.dtype], *ctx.layout, ids.data_ptr(), stats.data_ptr(), grad_output.data_ptr(),
+                ctx.temperature, grad.data_ptr(), grad.shape[-1], ids.numel(), grad.shape[-1],
                 _native.stream_handle(rows.device)))
-        return grad.reshape(ctx.shape), None, None
+        return grad, None, None
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
     """``log_softmax(logits / temperature)[..., token_ids]`` in fp32, differentiable with respect to the logits.
 
-    ``logits`` is ``[..., vocab]`` in bf16 or fp32 (any row stride), ``token_ids`` int64 of the leading shape.  A token id
+    ``logits`` is ``[..., vocab]`` in bf16 or fp32 (a slice such as ``logits[:, :-1]`` is read where it is), ``token_ids`` int64 of the leading shape.  A token id
     outside ``[0, vocab)`` (an ignore index such as -100) gives 0 and no gradient, whatever its row holds.  Logits of -inf
     have probability zero; a row without a finite logit, or with a NaN or +inf, gives NaN."""
     _check(logits, token_ids)
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogprobs.apply(logits, token_ids, float(temperature))
-    return _forward(_rows(logits), token_ids.contiguous(), float(temperature), None)
+    return _forward(*_read_where_it_is(logits), token_ids.contiguous(), float(temperature), None)
 
 
 def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -96,7 +108,7 @@ def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weig
     be ``logits`` itself, which it then overwrites (it must not overlap them in any other way).  Nothing is recorded for
     autograd."""
     dtype = _check(logits, token_ids)
-    rows, ids = _rows(logits.detach()), token_ids.contiguous()
+    (rows, layout), ids = _read_where_it_is(logits.detach()), token_ids.contiguous()
     if weight is not None:
         if weight.shape != token_ids.shape or weight.dtype != torch.float32 or weight.device != logits.device:
             raise ValueError("weight must be float32 of the shape of token_ids on the logits' device")
@@ -118,7 +130,7 @@ def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weig
     logprobs = torch.empty(token_ids.shape, dtype=torch.float32, device=logits.device)
     with _native.on_device(logits.device):
         _native.check(_native.library().molt_token_logprob_grad(
-            rows.data_ptr(), dtype, _stride(rows), ids.data_ptr(), _native.ptr(weight), float(temperature), logprobs.data_ptr(),
-            target.data_ptr(), _stride(target), rows.shape[0], rows.shape[1], _native.stream_handle(logits.device)))
+            rows.data_ptr(), dtype, *layout, ids.data_ptr(), _native.ptr(weight), float(temperature), logprobs.data_ptr(),
+            target.data_ptr(), _stride(target), ids.numel(), rows.shape[-1], _native.stream_handle(logits.device)))
     torch.autograd.graph.increment_version(out)
     return logprobs, out

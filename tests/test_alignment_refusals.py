@@ -36,35 +36,38 @@ def _refused(code, expected, word):
     ({"grad": C + 1}, _native.E_VALUE, "aligned"), ({"grad_stride": 99}, _native.E_VALUE, "overlap"),
     ({"grad_stride": 0}, _native.E_VALUE, "overlap"), ({"grad": A + 2}, _native.E_VALUE, "overlaps"),
     ({"grad": A, "grad_stride": 104}, _native.E_VALUE, "overlaps"), ({"grad": A + 2 * 50}, _native.E_VALUE, "overlaps"),
-    ({"grad": A - 2 * 300}, _native.E_VALUE, "overlaps")])
+    ({"grad": A - 2 * 300}, _native.E_VALUE, "overlaps"), ({"groups": (-1, 0)}, _native.E_VALUE, "group_rows"),
+    ({"groups": (2, 99)}, _native.E_VALUE, "groups"), ({"groups": (2, -200)}, _native.E_VALUE, "groups"),
+    ({"grad": A, "groups": (2, 300)}, _native.E_VALUE, "overlaps"), ({"grad": A + 2 * 700, "groups": (1, 300)}, _native.E_VALUE, "overlaps"),
+    ({"grad": A + 2 * 100, "stride": 200, "grad_stride": 200, "groups": (2, 500)}, _native.E_VALUE, "overlaps")])
 def test_token_logprob_refusals(native_library, change, expected, word):
     call = dict(logits=A, dtype=_native.DTYPE_BF16, stride=100, ids=B, temperature=1.0, logprob=D, grad=C, grad_stride=100,
-                rows=4, vocab=100)
+                rows=4, vocab=100, groups=(0, 0))
     call.update(change)
     c = call
     lib = native_library
-    _refused(lib.molt_token_logprob_grad(c["logits"], c["dtype"], c["stride"], c["ids"], None, c["temperature"], c["logprob"],
+    _refused(lib.molt_token_logprob_grad(c["logits"], c["dtype"], c["stride"], *c["groups"], c["ids"], None, c["temperature"], c["logprob"],
                                          c["grad"], c["grad_stride"], c["rows"], c["vocab"], 0), expected, word)
     if "logprob" not in change:
-        _refused(lib.molt_token_logprob_bwd(c["logits"], c["dtype"], c["stride"], c["ids"], E, E, c["temperature"], c["grad"],
+        _refused(lib.molt_token_logprob_bwd(c["logits"], c["dtype"], c["stride"], *c["groups"], c["ids"], E, E, c["temperature"], c["grad"],
                                             c["grad_stride"], c["rows"], c["vocab"], 0), expected, word)
     if not set(change) & {"grad", "grad_stride"}:
-        _refused(lib.molt_token_logprob_fwd(c["logits"], c["dtype"], c["stride"], c["ids"], c["temperature"], c["logprob"], None,
+        _refused(lib.molt_token_logprob_fwd(c["logits"], c["dtype"], c["stride"], *c["groups"], c["ids"], c["temperature"], c["logprob"], None,
                                             c["rows"], c["vocab"], 0), expected, word)
 
 
 def test_token_logprob_stats_are_aligned(native_library):
     lib = native_library
-    _refused(lib.molt_token_logprob_fwd(A, 0, 100, B, 1.0, D, E + 4, 4, 100, 0), _native.E_VALUE, "stats")
-    _refused(lib.molt_token_logprob_bwd(A, 0, 100, B, E + 4, E, 1.0, C, 100, 4, 100, 0), _native.E_VALUE, "stats")
+    _refused(lib.molt_token_logprob_fwd(A, 0, 100, 0, 0, B, 1.0, D, E + 4, 4, 100, 0), _native.E_VALUE, "stats")
+    _refused(lib.molt_token_logprob_bwd(A, 0, 100, 0, 0, B, E + 4, E, 1.0, C, 100, 4, 100, 0), _native.E_VALUE, "stats")
 
 
 def test_token_logprob_of_no_rows_is_no_launch(native_library):
     lib = native_library
     before = lib.molt_launch_count()
-    assert lib.molt_token_logprob_fwd(None, 0, 0, None, 1.0, None, None, 0, 10, 0) == 0
-    assert lib.molt_token_logprob_grad(None, 0, 0, None, None, 1.0, None, None, 0, 0, 10, 0) == 0
-    assert lib.molt_token_logprob_bwd(None, 0, 0, None, None, None, 1.0, None, 0, 0, 10, 0) == 0
+    assert lib.molt_token_logprob_fwd(None, 0, 0, 0, 0, None, 1.0, None, None, 0, 10, 0) == 0
+    assert lib.molt_token_logprob_grad(None, 0, 0, 0, 0, None, None, 1.0, None, None, 0, 0, 10, 0) == 0
+    assert lib.molt_token_logprob_bwd(None, 0, 0, 0, 0, None, None, None, 1.0, None, 0, 0, 10, 0) == 0
     assert lib.molt_launch_count() == before
 
 

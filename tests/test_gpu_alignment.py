@@ -185,6 +185,60 @@ def test_token_logprobs_shapes_strides_and_offsets(native_library):
     assert torch.equal(a, b) and torch.equal(g, h)
 
 
+GROUPED = {
+    "all but the last": lambda x: x[:, :-1],
+    "every second": lambda x: x[:, ::2],
+    "batch last": lambda x: x.transpose(0, 1),
+    "one batch for all": lambda x: x[:1].expand(5, -1, -1),
+    "one row per batch": lambda x: x[:, :1].expand(-1, 4, -1),
+    "inner columns": lambda x: x[1:, 1:-1, 3:-2],
+    "four dimensions": lambda x: x[:, :-1].unflatten(1, (2, -1))[:, :, :2],     # three strides: a copy
+    "a row each": lambda x: x[:, 2],
+}
+
+
+@pytest.mark.parametrize("form", GROUPED)
+@pytest.mark.parametrize("vocab", [37, 5000, 40000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_token_logprobs_of_rows_in_groups(native_library, form, vocab, dtype):
+    from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
+
+    gen = _gen(vocab + len(form))
+    store = (torch.randn(3, 7, vocab, device="cuda", generator=gen) * 2).to(dtype)
+    logits = GROUPED[form](store)
+    shape, width = logits.shape[:-1], logits.shape[-1]
+    ids = torch.randint(0, width, shape, device="cuda", generator=gen)
+    ids.view(-1)[1] = -100
+    weight = torch.randn(shape, device="cuda", generator=gen)
+    flat, w = ids.reshape(-1), weight.reshape(-1)
+    want, probs, kept, bound = _exact_logprobs(logits.reshape(-1, width), flat, 0.7)
+    want_grad = _exact_grad(probs, flat, kept, w, 0.7)
+    assert token_logprobs(logits, ids, 0.7).shape == shape
+    _close(token_logprobs(logits, ids, 0.7).reshape(-1), want, bound)
+    leaf = logits.detach().requires_grad_()
+    lp = token_logprobs(leaf, ids, 0.7)
+    _close(lp.detach().reshape(-1), want, bound)
+    (grad,) = torch.autograd.grad(lp, leaf, weight)
+    assert grad.shape == logits.shape
+    _check_grad(grad.reshape(-1, width), want_grad, bound, w, 0.7, dtype)
+    lp, grad = token_logprobs_with_grad(logits, ids, weight, 0.7)
+    assert lp.shape == shape and grad.shape == logits.shape
+    _close(lp.reshape(-1), want, bound)
+    _check_grad(grad.reshape(-1, width), want_grad, bound, w, 0.7, dtype)
+
+
+def test_token_logprobs_make_no_copy_of_a_slice(native_library):
+    from molt_b200.kernels import token_logprobs
+
+    logits = torch.zeros(4, 65, 40000, device="cuda", dtype=torch.bfloat16)
+    ids = torch.zeros(4, 64, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    token_logprobs(logits[:, :-1], ids)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+
+
 def _check_all_forms(logits, ids, temperature, out=None):
     from molt_b200.kernels import token_logprobs, token_logprobs_with_grad
 
