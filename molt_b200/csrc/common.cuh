@@ -95,9 +95,23 @@ __device__ __forceinline__ float load_absmax(const WeightView& w, long long blk)
 
 // Programmatic dependence of two kernels in a stream: the second one's blocks are brought up while the first one ends.  The
 // first calls let_next_begin(), the second is launched by launch_behind() and calls wait_for_previous() before it reads what
-// the first wrote (all of the first has then run and can be seen).
+// the first wrote (all of the first has then run and can be seen).  Until the wait that data changes while the second one
+// lives, so the second must not take it through a const __restrict__ pointer, whose loads the compiler may serve from a cache
+// that is not coherent or move in front of the wait: it takes partial sums as Written.
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// 64-bit values that the previous kernel of the stream has written.  The loads are volatile like the wait, and so stay
+// behind it, and they read the L2.
+struct Written {
+  const double* values;
+  __host__ __device__ Written(const double* p) : values(p) {}
+  __device__ __forceinline__ double operator[](long long i) const {
+    double v;
+    asm volatile("ld.relaxed.gpu.global.f64 %0, [%1];" : "=d"(v) : "l"(values + i));
+    return v;
+  }
+};
 
 template <typename... Params, typename... Args>
 inline void launch_behind(void (*kernel)(Params...), unsigned blocks, unsigned threads, cudaStream_t s, const Args&... args) {

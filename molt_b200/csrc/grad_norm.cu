@@ -186,9 +186,15 @@ __global__ void __launch_bounds__(kThreads, 5) norm_kernel(const __grid_constant
 
 // The norm and the coefficient from the partial sums, by one block; every thread gets them.
 template <bool MAX>
-__device__ __forceinline__ float2 finish(const double* __restrict__ part, int parts, float grad_scale, float max_norm) {
+__device__ __forceinline__ float2 finish(const Written part, int parts, float grad_scale, float max_norm) {
   double acc = 0.;
-  for (int i = threadIdx.x; i < parts; i += blockDim.x) acc = MAX ? larger(acc, part[i]) : acc + part[i];
+  for (int i = threadIdx.x; i < parts; i += kUnroll * blockDim.x) {
+    double v[kUnroll];   // all requested before the first is used: volatile loads are not moved together
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) v[j] = i + j * blockDim.x < parts ? part[i + j * blockDim.x] : 0.;
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) acc = MAX ? larger(acc, v[j]) : acc + v[j];
+  }
   acc = block_total<MAX>(acc);
   const float norm = (float)((MAX ? acc : sqrt(acc)) * fabs((double)grad_scale));
   const float c = max_norm / (norm + 1e-6f);
@@ -196,7 +202,7 @@ __device__ __forceinline__ float2 finish(const double* __restrict__ part, int pa
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* __restrict__ part, int parts, float grad_scale,
+__global__ void __launch_bounds__(kThreads) norm_finish_kernel(const Written part, int parts, float grad_scale,
                                                                float max_norm, float* __restrict__ result) {
   wait_for_previous();
   const float2 r = finish<MAX>(part, parts, grad_scale, max_norm);
@@ -239,7 +245,7 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int n, float c) 
 // written take 220 us (6.7 TB/s), the 74 MB arena 22 us.
 template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<CAPACITY> table,
-                                                         const double* __restrict__ part, int parts, float max_norm,
+                                                         const Written part, int parts, float max_norm,
                                                          float* __restrict__ result) {
   wait_for_previous();
   const float2 r = finish<MAX>(part, parts, 1.f, max_norm);

@@ -101,10 +101,11 @@ constexpr int kWarpRows = 2048, kWarpTokens = kRound, kWarps = kThreads / 32;
 bool warp_rows(int64_t rows, int64_t seq) { return rows >= kWarpRows && seq <= kWarpTokens; }
 int warp_row_blocks(int64_t rows) { return (int)((rows + kWarps - 1) / kWarps < 148 * 8 ? (rows + kWarps - 1) / kWarps : 148 * 8); }
 
-// Sums over the splits of row b of its N values.  A row of many splits is added up by a warp, whose lanes all call this.
+// Sums over the splits of row b of its N values, which lie in shared memory or were Written by the kernel before.  A row of many
+// splits is added up by a warp, whose lanes all call this.
 constexpr int kSplitsPerThread = 8;
-template <int N>
-__device__ __forceinline__ void row_sums(const double* part, long long b, int splits, double (&row)[N]) {
+template <int N, typename Part>
+__device__ __forceinline__ void row_sums(const Part& part, long long b, int splits, double (&row)[N]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < N; ++i) row[i] = 0.;
@@ -258,7 +259,8 @@ __device__ __forceinline__ void policy_result(double (&sum)[4], double kl_coef, 
 }
 
 // Rows, their weights and the result, by one block.
-__device__ __forceinline__ void policy_finish(const double* part, long long batch, int splits, int reduction, double kl_coef,
+template <typename Part>
+__device__ __forceinline__ void policy_finish(const Part& part, long long batch, int splits, int reduction, double kl_coef,
                                               float* __restrict__ row_weight, float* __restrict__ loss,
                                               float* __restrict__ stats) {
   double sum[4] = {0., 0., 0., 0.};
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 5) policy_kernel(PolicyArgs a, float
   if ((threadIdx.x & 31) == 0 && value < 4) part[(b * a.splits + blockIdx.y) * 4 + value] = mine;
 }
 
-__global__ void __launch_bounds__(kFinish) policy_finish_kernel(const double* __restrict__ part, long long batch, int splits,
+__global__ void __launch_bounds__(kFinish) policy_finish_kernel(const Written part, long long batch, int splits,
                                                              int reduction, double kl_coef, float* __restrict__ row_weight,
                                                              float* __restrict__ loss, float* __restrict__ stats) {
   wait_for_previous();
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 4) policy_rows_kernel(PolicyArgs a, 
   if (lane == 0 && warp < 4) part[blockIdx.x * 4 + warp] = mine;
 }
 
-__global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const double* __restrict__ part, int blocks, double kl_coef,
+__global__ void __launch_bounds__(kFinish) policy_rows_finish_kernel(const Written part, int blocks, double kl_coef,
                                                                      float* __restrict__ scale, float* __restrict__ loss,
                                                                      float* __restrict__ stats) {
   wait_for_previous();
@@ -437,7 +439,8 @@ __device__ __forceinline__ void preference_tokens(const PreferenceArgs& a, long 
   if (t0 < end) round(t0, Ragged{});
 }
 
-__device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const double* part, float* __restrict__ seq_grad,
+template <typename Part>
+__device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const Part& part, float* __restrict__ seq_grad,
                                                   float* __restrict__ rewards, float* __restrict__ loss_out) {
   double total[1] = {0.};
   for (long long p = first_row(a.splits); p < a.pairs; p += row_step(a.splits)) {
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 8) preference_rows_kernel(Preference
   }
 }
 
-__global__ void __launch_bounds__(kFinish) preference_finish_kernel(PreferenceArgs a, const double* __restrict__ part,
+__global__ void __launch_bounds__(kFinish) preference_finish_kernel(PreferenceArgs a, const Written part,
                                                                  float* __restrict__ seq_grad, float* __restrict__ rewards,
                                                                  float* __restrict__ loss) {
   wait_for_previous();
