@@ -210,9 +210,10 @@ __device__ __forceinline__ void policy_tokens(const PolicyArgs& a, long long b, 
       ratio(d, r, less);
       // -r A as -A, added in 64 bits, and -(r - 1) A, which is small near the policy that sampled: advantages of both signs
       // cancel in the mean, the rounding of products of order one would not.  The product with an advantage of zero is zero
-      // however large the ratio (NaN stays NaN).
-      const float rest = adv[j] == 0.f ? 0.f : -(cut ? (adv[j] > 0.f ? a.above : a.below) : less) * adv[j];
-      float g = cut || adv[j] == 0.f ? 0.f : -r * adv[j];
+      // however large the ratio; a NaN stays one.
+      const bool nothing = adv[j] == 0.f && !isnan(d);
+      const float rest = nothing ? 0.f : -(cut ? (adv[j] > 0.f ? a.above : a.below) : less) * adv[j];
+      float g = cut || nothing ? 0.f : -r * adv[j];
       if (REF) {
         float k, slope;
         divergence(ref[j] - lp[j], k, slope);
