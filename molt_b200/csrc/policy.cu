@@ -461,7 +461,9 @@ __device__ __forceinline__ void preference_finish(const PreferenceArgs& a, const
     double loss, slope;
     if (a.kind == MOLT_PREFERENCE_SIGMOID) {
       const double z = a.beta * h, e = exp(-fabs(z)), soft = log1p(e);   // -ln sig(z) = soft + max(-z, 0)
-      loss = soft + (1. - a.smoothing) * fmax(-z, 0.) + a.smoothing * fmax(z, 0.);
+      loss = soft;                                                       // an infinite z must not meet a factor of zero
+      if (a.smoothing != 1.) loss += (1. - a.smoothing) * fmax(-z, 0.);
+      if (a.smoothing != 0.) loss += a.smoothing * fmax(z, 0.);
       if (isnan(z)) loss = z;
       const double small = e / (1. + e), large = 1. / (1. + e);          // sig(-|z|), sig(|z|)
       slope = -a.beta * ((1. - a.smoothing) * (z >= 0. ? small : large) - a.smoothing * (z >= 0. ? large : small));

@@ -34,3 +34,30 @@ def test_policy_loss_keeps_a_nan_beside_an_advantage_of_zero(native_library, bat
         if masked:
             assert float(got.loss) == 0.0
         assert float(got.clip_fraction) == 0.0
+
+
+@pytest.mark.parametrize("pairs,seq", [(2, 3), (400, 40), (1100, 7)])     # one block, a block per row, a warp per row
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 1.0])
+def test_preference_loss_of_sequences_without_probability(native_library, pairs, seq, smoothing):
+    """A kept token of probability zero in the rejected sequence: -ln sig(inf) = 0, and with smoothing infinite; in the chosen
+    one the other way round.  The slope has its limits 0, beta e and -beta (1 - e).  Other pairs keep their share."""
+    from molt_b200.kernels import preference_loss
+
+    beta = 0.5
+    one = -(1 - smoothing) * math.log(0.5) - smoothing * math.log(0.5)          # a pair with h = 0
+    for side in ("rejected", "chosen"):
+        lp = torch.full((2 * pairs, seq), -1.0, device="cuda")
+        lp[pairs if side == "rejected" else 0, seq - 1] = -math.inf
+        leaf = lp.requires_grad_()
+        got = preference_loss(leaf, beta=beta, label_smoothing=smoothing)
+        (grad,) = torch.autograd.grad(got.loss, leaf)
+        against = smoothing if side == "rejected" else 1.0 - smoothing          # the factor of the infinite term
+        want = math.inf if against else one * (pairs - 1) / pairs
+        # the loss is summed in 64 bits and rounded once, the logarithm above is off by 2^-53
+        assert float(got.loss) == pytest.approx(want, rel=2.0 ** -23, abs=0.0)
+        slope = (beta * smoothing if side == "rejected" else -beta * (1.0 - smoothing)) / pairs
+        for row, sign in ((0, 1.0), (pairs, -1.0)):
+            assert torch.equal(grad[row], grad[row, :1].expand(seq))
+            assert float(grad[row, 0]) == pytest.approx(sign * slope, rel=2.0 ** -23, abs=0.0)
+        at = got.rejected_rewards if side == "rejected" else got.chosen_rewards
+        assert float(at[0]) == -math.inf and bool(at[1:].isfinite().all())
