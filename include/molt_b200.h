@@ -398,8 +398,9 @@ typedef struct molt_grad_item {
 
 /* Global norm of a list of gradients (items: array in HOST memory, read before the call returns) and the clipping
  * coefficient: result[0] = norm of |grad_scale| * g over all elements, result[1] = min(1, max_norm / (result[0] + 1e-6)).
- * Squares that leave fp32's range are added in 64 bits, so the norm is right for every finite gradient; a NaN or an
- * infinity reaches result[0].  Same bits for the same list on every call. */
+ * Squares that leave fp32's range are added in 64 bits, and the coefficient is formed from the 64-bit norm.  A norm of finite
+ * gradients beyond fp32's range is reported as FLT_MAX; a NaN or an infinity among them reaches result[0], and only those do.
+ * Same bits for the same list on every call, at the same alignment of its tensors to 16 bytes. */
 size_t molt_grad_norm_workspace_bytes(int count);
 int molt_grad_norm(const molt_grad_item* items, int count, int norm_kind, float grad_scale, float max_norm, float* result,
                    void* workspace, size_t workspace_bytes, uintptr_t stream);

@@ -4,6 +4,7 @@
 // table is walked in several launches.  Every tensor is cut into chunks, the chunks of the list are numbered through, and
 // block i of G takes chunks i, i + G, ...; it leaves one partial sum, and the partial sums are added in a fixed order, so a
 // list gives the same bits on every call.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -196,9 +197,12 @@ __device__ __forceinline__ float2 finish(const Written part, int parts, float gr
     for (int j = 0; j < kUnroll; ++j) acc = MAX ? larger(acc, v[j]) : acc + v[j];
   }
   acc = block_total<MAX>(acc);
-  const float norm = (float)((MAX ? acc : sqrt(acc)) * fabs((double)grad_scale));
-  const float c = max_norm / (norm + 1e-6f);
-  return make_float2(norm, c > 1.f ? 1.f : c);   // NaN stays
+  // The norm of finite gradients may be beyond fp32: the coefficient comes from the 64-bit norm, and the norm is reported as
+  // fp32's largest value, so that only a gradient that is not finite gives a norm that is not.
+  const double norm = (MAX ? acc : sqrt(acc)) * fabs((double)grad_scale);
+  const double c = (double)max_norm / (norm + 1e-6);
+  const float reported = norm > (double)FLT_MAX && !isinf(norm) ? FLT_MAX : (float)norm;
+  return make_float2(reported, c > 1. ? 1.f : (float)c);   // NaN stays
 }
 
 template <bool MAX>

@@ -68,15 +68,16 @@ def _launch(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, 
 
 def global_grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of ``grads`` (one tensor or a sequence; bf16 and fp32 may be mixed) as an fp32 scalar on the
-    device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  It is right for every
-    finite gradient, however large or small; a NaN gives NaN, and an infinity infinity.  Equal lists give equal bits.
-    Nothing is recorded for autograd."""
+    device: the square root of the sum of squares (``norm_type`` 2) or the largest magnitude (``inf``).  Squares of any finite
+    gradient are held; a norm beyond fp32's range is reported as fp32's largest value.  A NaN gives NaN, and an infinity
+    infinity.  Equal lists of equal alignment (to 16 bytes) give equal bits.  Nothing is recorded for autograd."""
     grads, _ = _checked("grads", grads)
     return _launch(grads, None, _norm_kind(norm_type), float("inf"))
 
 
 def clip_grad_norm(grads: Grads, max_norm: float, norm_type: float = 2.0, out: Optional[Grads] = None) -> torch.Tensor:
-    """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return their :func:`global_grad_norm` before that.
+    """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return their :func:`global_grad_norm` before that.  The
+    factor is formed from the norm in 64 bits, so finite gradients are clipped rightly where their norm leaves fp32 too.
 
     In place, or into ``out``: tensors of the same dtypes and sizes that lie in memory as ``grads`` do (of contiguous ones the
     shapes may differ).  An output may be its own gradient but must not overlap another tensor of the call.  One tensor must

@@ -61,3 +61,45 @@ def test_preference_loss_of_sequences_without_probability(native_library, pairs,
             assert float(grad[row, 0]) == pytest.approx(sign * slope, rel=2.0 ** -23, abs=0.0)
         at = got.rejected_rewards if side == "rejected" else got.chosen_rewards
         assert float(at[0]) == -math.inf and bool(at[1:].isfinite().all())
+
+
+@pytest.mark.parametrize("values", [[3e38, 3e38], [3.3e38] * 5000, [-3e38, 1.0, 2e38, 0.0, 1e-30]], ids=["two", "many", "mixed"])
+def test_clipping_by_a_norm_beyond_fp32(native_library, values):
+    """Finite gradients whose norm no fp32 value can hold.  The norm is reported as fp32's largest value; the coefficient
+    comes from the norm in 64 bits: off by half a step of its own, 2^-150 where it is subnormal, 2^-24 of it where not.  The
+    norm itself is off by 2^-20 at most (squares in 64 bits throughout here, so far less), the product by one rounding."""
+    from molt_b200.kernels import clip_grad_norm, global_grad_norm
+
+    top = torch.finfo(torch.float32).max
+    grad = torch.tensor(values, device="cuda")
+    exact = grad.double()
+    norm = exact.norm()
+    assert float(norm) > top
+    assert float(global_grad_norm([grad])) == top
+    for max_norm in (1.0, 1e30, 3e38):
+        out = torch.empty_like(grad)
+        assert float(clip_grad_norm([grad], max_norm, out=[out])) == top
+        limit = float(torch.tensor(max_norm).float())
+        coefficient = limit / float(norm)
+        step = max(2.0 ** -150, coefficient * 2.0 ** -24)
+        bound = exact.abs() * (step + coefficient * 2.0 ** -20) + 2.0 ** -150
+        assert bool(((out.double() - exact * coefficient).abs() <= bound).all())
+    out = torch.empty_like(grad)
+    clip_grad_norm([grad], math.inf, out=[out])
+    assert torch.equal(out, grad)
+    for bad in (math.inf, math.nan):                       # these are still told apart
+        assert not math.isfinite(float(global_grad_norm([grad, torch.tensor([bad], device="cuda")])))
+
+
+def test_clipped_optimizer_step_with_a_norm_beyond_fp32(native_library):
+    """Two gradients of 3e38 clipped to 1e15 (1e15 / sqrt(2) each, whose squares fp32 holds).  The first AdamW step from
+    moments of zero moves a parameter by lr g / (|g| + eps): 16 roundings of 2^-24 at most, eps is below 2^-70 of |g|."""
+    from molt_b200.data_parallel import GradArena, ParamArena
+
+    p = torch.nn.Parameter(torch.zeros(2, device="cuda"))
+    grads = GradArena([p])
+    opt = ParamArena(grads, lr=0.5)
+    grads.views[0].fill_(3e38)
+    norm = opt.step(max_norm=1e15)
+    assert math.isfinite(float(norm))
+    assert bool(((p.detach() + 0.5).abs() <= 0.5 * 16 * 2.0 ** -24).all())
