@@ -410,10 +410,18 @@ int molt_clip_grads(const molt_grad_item* items, int count, int norm_kind, float
                     size_t workspace_bytes, uintptr_t stream);
 
 /* molt_adamw_step whose gradients are also multiplied by clip[1], clip being the result of molt_grad_norm with the same
- * grad_scale (device memory; nothing waits on the host).  A step whose norm clip[0] is not finite changes nothing. */
+ * grad_scale (device memory; nothing waits on the host).  A step whose norm clip[0] is not finite changes neither
+ * parameters nor moments.  The bias corrections are those of `step` as given: whoever does not learn which steps were left
+ * out uses molt_adamw_step_counted. */
 int molt_adamw_step_clipped(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count, float lr,
                             float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
                             const float* clip, uintptr_t stream);
+/* The same with a count of the steps that were left out, skipped[0] (device memory, 8-byte aligned, zero at first, the same for
+ * every step over these moments): a step without a finite norm adds one to it and changes nothing else, and the bias
+ * corrections of the others are those of step - skipped[0].  clip may be NULL (no clipping; nothing is left out). */
+int molt_adamw_step_counted(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count, float lr,
+                            float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
+                            const float* clip, int64_t* skipped, uintptr_t stream);
 
 #ifdef __cplusplus
 }

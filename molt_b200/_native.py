@@ -44,6 +44,7 @@ EXPORTS = (
     "molt_token_logprob_grad", "molt_policy_loss_workspace_bytes", "molt_policy_loss_fwd", "molt_policy_loss_bwd",
     "molt_preference_loss_workspace_bytes", "molt_preference_loss_fwd", "molt_preference_loss_bwd",
     "molt_grad_norm_workspace_bytes", "molt_grad_norm", "molt_clip_grads", "molt_adamw_step_clipped",
+    "molt_adamw_step_counted",
 )
 
 
@@ -204,6 +205,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.molt_clip_grads.argtypes = [vp, i32, i32, f32, vp, vp, sz, up]
     lib.molt_adamw_step_clipped.restype = i32
     lib.molt_adamw_step_clipped.argtypes = [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i64, f32, vp, up]
+    lib.molt_adamw_step_counted.restype = i32
+    lib.molt_adamw_step_counted.argtypes = [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i64, f32, vp, vp, up]
 
 
 def library() -> ctypes.CDLL:

@@ -404,14 +404,39 @@ __global__ void __launch_bounds__(256) rope_kernel(const __nv_bfloat16* q, const
 // AdamW over flat fp32 arrays (decoupled weight decay, bias correction as torch.optim.AdamW computes it).
 // All adapter parameters, their gradients and both moments live in flat arenas, so one launch steps every adapter.
 // ------------------------------------------------------------------------------------------------
+// A clipped step without a finite norm is left out, which only the device knows: `skipped` counts those steps, and the bias
+// corrections of later ones are those of the steps that were made.
+__device__ __forceinline__ double whole_power(double base, long long n) {
+  double r = 1.0;
+  for (; n > 0; n >>= 1, base *= base)
+    if (n & 1) r *= base;
+  return r;
+}
+
 __global__ void __launch_bounds__(256) adamw_kernel(float4* __restrict__ param, const float4* __restrict__ grad,
                                                     float4* __restrict__ exp_avg, float4* __restrict__ exp_avg_sq,
                                                     long long vectors, float lr, float beta1, float beta2, float eps,
-                                                    float weight_decay, float bias1, float bias2_sqrt, float grad_scale,
-                                                    const float* __restrict__ clip) {
+                                                    float weight_decay, long long step, float bias1, float bias2_sqrt,
+                                                    float grad_scale, const float* __restrict__ clip, long long* skipped) {
   if (clip != nullptr) {               // {global norm, clipping coefficient}
-    if (!isfinite(clip[0])) return;    // the step is left out: its gradients would poison both moments
+    if (!isfinite(clip[0])) {          // the step is left out: its gradients would poison both moments
+      if (skipped != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *skipped += 1;   // no other thread reads it in such a step
+      return;
+    }
     grad_scale *= clip[1];
+  }
+  if (skipped != nullptr) {
+    const long long made = step - *skipped;
+    if (made != step) {                // bias1 and bias2_sqrt are the host's, of `step`
+      __shared__ float corrected[2];
+      if (threadIdx.x == 0) {
+        corrected[0] = (float)(1.0 - whole_power(beta1, made));
+        corrected[1] = (float)sqrt(1.0 - whole_power(beta2, made));
+      }
+      __syncthreads();
+      bias1 = corrected[0];
+      bias2_sqrt = corrected[1];
+    }
   }
   for (long long v = blockIdx.x * (long long)blockDim.x + threadIdx.x; v < vectors;
        v += (long long)gridDim.x * blockDim.x) {
@@ -636,7 +661,7 @@ extern "C" int molt_rope(const void* q, const void* k, void* q_out, void* k_out,
 
 static int adamw_launch(const char* who, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
                         float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
-                        const float* clip, uintptr_t stream) {
+                        const float* clip, int64_t* skipped, uintptr_t stream) {
   MOLT_REQUIRE(param && grad && exp_avg && exp_avg_sq, MOLT_E_VALUE, "%s: NULL tensor pointer", who);
   MOLT_REQUIRE(count >= 0 && count % 4 == 0, MOLT_E_VALUE, "%s: the element count must be a multiple of 4", who);
   MOLT_REQUIRE(aligned16(param) && aligned16(grad) && aligned16(exp_avg) && aligned16(exp_avg_sq), MOLT_E_VALUE,
@@ -648,8 +673,8 @@ static int adamw_launch(const char* who, float* param, const float* grad, float*
   const long long vectors = count / 4;
   adamw_kernel<<<grid_for(vectors, 256, 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       reinterpret_cast<float4*>(param), reinterpret_cast<const float4*>(grad), reinterpret_cast<float4*>(exp_avg),
-      reinterpret_cast<float4*>(exp_avg_sq), vectors, lr, beta1, beta2, eps, weight_decay, (float)bias1,
-      (float)sqrt(bias2), grad_scale, clip);
+      reinterpret_cast<float4*>(exp_avg_sq), vectors, lr, beta1, beta2, eps, weight_decay, step, (float)bias1,
+      (float)sqrt(bias2), grad_scale, clip, reinterpret_cast<long long*>(skipped));
   return launch_status("adamw_kernel");
 }
 
@@ -657,7 +682,7 @@ extern "C" int molt_adamw_step(float* param, const float* grad, float* exp_avg, 
                                float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
                                float grad_scale, uintptr_t stream) {
   return adamw_launch("molt_adamw_step", param, grad, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, weight_decay, step,
-                      grad_scale, nullptr, stream);
+                      grad_scale, nullptr, nullptr, stream);
 }
 
 extern "C" int molt_adamw_step_clipped(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
@@ -665,7 +690,16 @@ extern "C" int molt_adamw_step_clipped(float* param, const float* grad, float* e
                                        float grad_scale, const float* clip, uintptr_t stream) {
   MOLT_REQUIRE(clip != nullptr, MOLT_E_VALUE, "molt_adamw_step_clipped: clip is NULL");
   return adamw_launch("molt_adamw_step_clipped", param, grad, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, weight_decay,
-                      step, grad_scale, clip, stream);
+                      step, grad_scale, clip, nullptr, stream);
+}
+
+extern "C" int molt_adamw_step_counted(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t count,
+                                       float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
+                                       float grad_scale, const float* clip, int64_t* skipped, uintptr_t stream) {
+  MOLT_REQUIRE(skipped != nullptr && reinterpret_cast<uintptr_t>(skipped) % 8 == 0, MOLT_E_VALUE,
+               "molt_adamw_step_counted: skipped is NULL or not 8-byte aligned");
+  return adamw_launch("molt_adamw_step_counted", param, grad, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, weight_decay,
+                      step, grad_scale, clip, skipped, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -129,7 +129,7 @@ class GradArena:
 
 class ParamArena:
     """The parameters themselves in one flat fp32 buffer, laid out exactly like a :class:`GradArena` over the same list
-    (same offsets), with the two AdamW moments beside it: one fused kernel (``molt_adamw_step``) then steps every
+    (same offsets), with the two AdamW moments beside it: one fused kernel (``molt_adamw_step_counted``) then steps every
     adapter of the model.  Takes the place of the per-parameter optimizer the reference builds
     (reference training/qlora.py:218-243) and steps (:982-986)."""
 
@@ -145,7 +145,8 @@ class ParamArena:
         self.exp_avg = torch.zeros_like(self.flat)
         self.exp_avg_sq = torch.zeros_like(self.flat)
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), betas, float(eps), float(weight_decay)
-        self.steps = 0
+        self.steps = 0                          # calls of step()
+        self.skipped = torch.zeros(1, dtype=torch.int64, device=self.flat.device)   # those of them that were left out
 
     def step(self, grad_scale: float = 1.0, max_norm: Optional[float] = None) -> Optional[torch.Tensor]:
         """One AdamW step over every parameter, on the current stream.
@@ -153,7 +154,7 @@ class ParamArena:
         With ``max_norm`` the gradients (times ``grad_scale``) are clipped to that global norm inside the optimizer's pass:
         one kernel more reads them for the norm, none rewrites them.  Returns the norm before clipping, a scalar on the
         device (after a summing all-reduce every rank finds the same one); a step whose norm is not finite changes
-        neither parameters nor moments."""
+        neither parameters nor moments, and later bias corrections do not count it (``skipped`` does, on the device)."""
         from molt_b200 import _native
 
         if max_norm is not None and not max_norm >= 0.0:
@@ -167,14 +168,14 @@ class ParamArena:
         with torch.cuda.device(flat.device):
             stream = _native.stream_handle(flat.device)
             if max_norm is None:
-                _native.check(lib.molt_adamw_step(*arguments, stream))
+                _native.check(lib.molt_adamw_step_counted(*arguments, None, self.skipped.data_ptr(), stream))
                 return None
             item = _native.grad_items((self.grads.flat,))
             clip = torch.empty(2, dtype=torch.float32, device=flat.device)
             scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(1), flat.device)
             _native.check(lib.molt_grad_norm(item.buffer_info()[0], 1, _native.NORM_L2, float(grad_scale), float(max_norm),
                                              clip.data_ptr(), scratch.data_ptr(), scratch.numel(), stream))
-            _native.check(lib.molt_adamw_step_clipped(*arguments, clip.data_ptr(), stream))
+            _native.check(lib.molt_adamw_step_counted(*arguments, clip.data_ptr(), self.skipped.data_ptr(), stream))
         return clip[0]
 
 

@@ -103,3 +103,48 @@ def test_clipped_optimizer_step_with_a_norm_beyond_fp32(native_library):
     norm = opt.step(max_norm=1e15)
     assert math.isfinite(float(norm))
     assert bool(((p.detach() + 0.5).abs() <= 0.5 * 16 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("bad_at", [(0,), (2,), (0, 1, 3), (5,)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_step_left_out_does_not_count(native_library, bad_at, bad):
+    """A run with steps whose norm is not finite, against one that never saw them: the same moments, and parameters that
+    differ only where a bias correction formed on the device is rounded to fp32 another way than the host's (2^-23 of it, and
+    so at most 2^-22 of a step's change for both).  A change is below 4 lr: m / sqrt(v) of six random gradients is below 1.1
+    by Cauchy and Schwarz, and the weight decay adds 0.1 |p|.  A parameter is rounded twice a step, from values that may then
+    differ: 2^-23 of it each time."""
+    from molt_b200.data_parallel import GradArena, ParamArena
+
+    def arena():
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        params = [torch.nn.Parameter(torch.randn(n, device="cuda", generator=gen)) for n in (1000, 5)]
+        return GradArena(params), params
+
+    lr, gen = 1e-2, torch.Generator(device="cuda").manual_seed(4)
+    batches = [torch.randn(1005, device="cuda", generator=gen) for _ in range(6)]
+    runs = []
+    for seen in (range(6), [i for i in range(6) if i not in bad_at]):
+        grads, params = arena()
+        opt = ParamArena(grads, lr=lr, weight_decay=0.1)
+        for i in seen:
+            grads.views[0].copy_(batches[i][:1000])
+            grads.views[1].copy_(batches[i][1000:])
+            if i in bad_at and len(seen) == 6:
+                grads.views[1][2] = bad
+            # the last step of all is made without a limit
+            opt.step(max_norm=None if i == 5 and i not in bad_at else 0.5)
+        runs.append((opt, torch.cat([p.detach() for p in params]), opt.exp_avg.clone(), opt.exp_avg_sq.clone()))
+    (_, p, m, v), (_, q, n, w) = runs
+    assert torch.equal(m, n) and torch.equal(v, w)
+    assert float((p - q).abs().max()) <= 6 * (4 * lr * 2.0 ** -22 + 2 * 2.0 ** -23 * float(q.abs().max()))
+
+
+def test_steps_left_out_are_counted_on_the_device(native_library):
+    from molt_b200.data_parallel import GradArena, ParamArena
+
+    grads = GradArena([torch.nn.Parameter(torch.ones(8, device="cuda"))])
+    opt = ParamArena(grads)
+    for value in (1.0, math.nan, math.inf, 1.0):
+        grads.views[0].fill_(value)
+        opt.step(max_norm=1.0)
+    assert opt.steps == 4 and opt.skipped.dtype == torch.int64 and opt.skipped.tolist() == [2]
