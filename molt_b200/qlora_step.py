@@ -500,10 +500,11 @@ def attach_lora_shadows(model: nn.Module) -> list:
 
 @contextmanager
 def leaves_of_its_own(model: nn.Module):
-    """Stand-ins for ``model``'s trainable parameters: the same memory, gradients and attributes, but other autograd leaves.
-    All graphs of a leaf share its accumulation node and the stream that the node was made on, so a backward pass that is
-    recorded while an eager graph of the same leaves is alive would reach out of the recording to that stream, which
-    ends the process.  A graph of stand-ins shares no node with one made before."""
+    """Stand-ins for ``model``'s trainable parameters: the same memory, gradients, attributes and tensor hooks, but other
+    autograd leaves.  All graphs of a leaf share its accumulation node and the stream that the node was made on, so a backward
+    pass that is recorded while an eager graph of the same leaves is alive would reach out of the recording to that stream,
+    which ends the process.  A graph of stand-ins shares no node with one made before; hooks that were registered on
+    such a node, instead of on the parameter, do not run."""
     held, stand_ins = [], {}
     for module in model.modules():
         for name, p in module._parameters.items():
@@ -515,11 +516,25 @@ def leaves_of_its_own(model: nn.Module):
                 other = stand_ins[p] = nn.Parameter(p.detach())
                 other.grad = p.grad
                 vars(other).update(vars(p))
+                for hook in list((p._backward_hooks or {}).values()):
+                    other.register_hook(hook)
+                for hook in list((p._post_accumulate_grad_hooks or {}).values()):
+                    other.register_post_accumulate_grad_hook(_with_parameter(hook, p))
             module._parameters[name] = stand_ins[p]
         yield
     finally:
         for module, name, p in held:
             module._parameters[name] = p
+
+
+def _with_parameter(hook, p):
+    """``hook`` of ``p``, called with ``p`` when the gradient of its stand-in has been accumulated."""
+    def call(other):
+        p.grad = other.grad
+        result = hook(p)
+        other.grad = p.grad
+        return result
+    return call
 
 
 class QLoRAStep:

@@ -1,6 +1,10 @@
 """Preference and policy tuning: refusals and host logic beside those of the operators' own tests."""
 from __future__ import annotations
 
+from contextlib import nullcontext
+
+import torch
+
 from molt_b200 import _native
 
 A, B, C, D, E = (0x10000 * i for i in range(1, 6))   # addresses that are only checked
@@ -13,3 +17,60 @@ def test_counted_adamw_needs_a_count(native_library):
     for change, word in (((A, B, C, D, 3), b"multiple of 4"), ((None, B, C, D, 4), b"NULL"), ((A + 4, B, C, D, 4), b"16-byte aligned")):
         rc = native_library.molt_adamw_step_counted(*change, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, None, E, 0)
         assert rc == _native.E_VALUE and word in native_library.molt_last_error()
+
+
+def _model(seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(3, 4), torch.nn.Linear(4, 2))
+
+
+def test_hooks_of_parameters_take_part_in_a_recording():
+    """Both kinds of tensor hooks, several on one parameter, a shared parameter, hooks taken off again: the gradients inside
+    are those of a backward pass outside, hooks run in the same order and get the parameter itself."""
+    from molt_b200.qlora_step import leaves_of_its_own
+
+    def triple(p):
+        p.grad.mul_(3)
+
+    x = torch.randn(5, 3)
+    runs = []
+    for inside in (False, True):
+        model = _model()
+        model.add_module("again", model[1])                       # the same parameters under two names
+        weight, bias, other = model[0].weight, model[0].bias, model[1].weight
+        told = []
+        weight.register_hook(lambda g: torch.full_like(g, 7.0))
+        weight.register_hook(lambda g: g * 2)
+        weight.register_hook(lambda g: g * 0).remove()
+        bias.register_post_accumulate_grad_hook(lambda p: told.append(p is bias))
+        bias.register_post_accumulate_grad_hook(triple)
+        bias.register_post_accumulate_grad_hook(lambda p: told.append("gone")).remove()
+        other.register_hook(lambda g: told.append("other"))
+        for p in model.parameters():
+            p.grad = torch.zeros_like(p)
+        grads = [p.grad for p in model.parameters()]
+        with leaves_of_its_own(model) if inside else nullcontext():
+            model[1](model[0](x)).square().sum().backward()
+        assert all(p.grad is g for p, g in zip(model.parameters(), grads))
+        assert told == ["other", True] and bool((weight.grad == 14).all())
+        runs.append([g.clone() for g in grads])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_hook_that_takes_the_gradient_away_does_so_in_a_recording():
+    """The optimizer inside the backward pass: the hook uses the parameter, and drops its gradient."""
+    from molt_b200.qlora_step import leaves_of_its_own
+
+    model = _model()
+    weight = model[0].weight
+    before = weight.detach().clone()
+
+    def step(p):
+        with torch.no_grad():
+            p.sub_(p.grad, alpha=0.1)
+        p.grad = None
+
+    weight.register_post_accumulate_grad_hook(step)
+    with leaves_of_its_own(model):
+        model(torch.randn(5, 3)).square().sum().backward()
+    assert weight.grad is None and not torch.equal(weight.detach(), before)

@@ -148,3 +148,33 @@ def test_steps_left_out_are_counted_on_the_device(native_library):
         grads.views[0].fill_(value)
         opt.step(max_norm=1.0)
     assert opt.steps == 4 and opt.skipped.dtype == torch.int64 and opt.skipped.tolist() == [2]
+
+
+def test_captured_step_runs_the_hooks_of_its_parameters(native_library):
+    """A weight that is trained beside the adapters, its gradient scaled by a hook: the captured steps give the eager ones'."""
+    from molt_b200.qlora_step import CrossEntropy, DecoderShape, QLoRAStep
+
+    shape = DecoderShape(layers=1, hidden=128, heads=4, kv_heads=2, head_dim=32, intermediate=256, vocab=512, rope_theta=1e4,
+                         rank=8, alpha=16.0, nested_absmax=True, seq_len=32, micro_batch=2)
+
+    class WithBias(CrossEntropy):
+        def loss(self, model, world, layer_done, tokens, targets):
+            return super().loss(model, world, layer_done, tokens, targets) + (model.bias * tokens.float().mean(0)).sum()
+
+    runs = []
+    for graph in (False, True):
+        step = QLoRAStep(shape, torch.device("cuda"), lr=1e-3, objective=WithBias(), cuda_graph=graph)
+        bias = step.model.bias = torch.nn.Parameter(torch.zeros(32, device="cuda"))
+        bias.grad = torch.zeros_like(bias)
+        bias.register_hook(lambda g: g * 3)
+        gen = torch.Generator(device="cuda").manual_seed(6)
+        grads = []
+        for _ in range(5):
+            tokens = torch.randint(0, 512, (2, 32), device="cuda", generator=gen)
+            bias.grad.zero_()
+            step.run(tokens, tokens.roll(-1, 1))
+            grads.append(bias.grad.clone())
+            assert torch.equal(grads[-1], 3 * tokens.float().mean(0))
+        assert (step.replayed_launches > 0) == graph
+        runs.append(torch.stack(grads))
+    assert torch.equal(*runs)
