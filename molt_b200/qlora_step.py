@@ -500,8 +500,8 @@ def attach_lora_shadows(model: nn.Module) -> list:
 
 @contextmanager
 def leaves_of_its_own(model: nn.Module):
-    """Stand-ins for ``model``'s trainable parameters: the same memory, gradients, attributes and tensor hooks, but other
-    autograd leaves.  All graphs of a leaf share its accumulation node and the stream that the node was made on, so a backward
+    """Stand-ins for ``model``'s trainable parameters: the same memory, gradients (those made inside are the parameters'
+    afterwards), attributes and tensor hooks, but other autograd leaves.  All graphs of a leaf share its accumulation node and the stream that the node was made on, so a backward
     pass that is recorded while an eager graph of the same leaves is alive would reach out of the recording to that stream,
     which ends the process.  A graph of stand-ins shares no node with one made before; hooks that were registered on
     such a node, instead of on the parameter, do not run."""
@@ -522,6 +522,9 @@ def leaves_of_its_own(model: nn.Module):
                     other.register_post_accumulate_grad_hook(_with_parameter(hook, p))
             module._parameters[name] = stand_ins[p]
         yield
+        for p, other in stand_ins.items():
+            if p.grad is None:               # made in here
+                p.grad = other.grad
     finally:
         for module, name, p in held:
             module._parameters[name] = p
@@ -600,6 +603,7 @@ class QLoRAStep:
         """Record forward + backward (+ the overlapped collectives) of one micro-batch once; every later step replays
         the recording (the kernels take raw pointers and never allocate or synchronise, so they are capture-safe)."""
         self._hold(*inputs)
+        self.arena.rebind()          # stand-ins begin with the gradients that their parameters have
         self._graph = torch.cuda.CUDAGraph()
         lib = _native.library()
         before = lib.molt_launch_count()

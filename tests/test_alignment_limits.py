@@ -3,6 +3,7 @@ from __future__ import annotations
 
 from contextlib import nullcontext
 
+import pytest
 import torch
 
 from molt_b200 import _native
@@ -74,3 +75,55 @@ def test_a_hook_that_takes_the_gradient_away_does_so_in_a_recording():
     with leaves_of_its_own(model):
         model(torch.randn(5, 3)).square().sum().backward()
     assert weight.grad is None and not torch.equal(weight.detach(), before)
+
+
+def test_gradients_made_in_a_recording_belong_to_the_parameters():
+    """A parameter that had no gradient has the recorded one afterwards, as after a backward pass without stand-ins."""
+    from molt_b200.qlora_step import leaves_of_its_own
+
+    model, plain = _model(), _model()
+    kept = model[0].weight.grad = torch.ones_like(model[0].weight)
+    plain[0].weight.grad = torch.ones_like(kept)
+    x = torch.randn(5, 3)
+    with leaves_of_its_own(model):
+        model(x).square().sum().backward()
+    plain(x).square().sum().backward()
+    assert model[0].weight.grad is kept
+    assert all(torch.equal(p.grad, q.grad) for p, q in zip(model.parameters(), plain.parameters()))
+
+
+class _Recording:
+    """Stands in for a CUDA graph: what runs inside is run."""
+
+    def replay(self):
+        raise AssertionError("nothing is replayed here")
+
+
+@pytest.fixture
+def host_step(monkeypatch, native_library):
+    from molt_b200.data_parallel import GradArena
+    from molt_b200.qlora_step import QLoRAStep
+
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _Recording)
+    monkeypatch.setattr(torch.cuda, "graph", lambda graph: nullcontext())
+    step = object.__new__(QLoRAStep)
+    step.model, step.world, step._graph, step._static_loss, step.graph_launches = _model(), 1, None, None, 0
+    step.arena = GradArena(step.model.parameters())
+
+    class Objective:
+        def loss(self, model, world, layer_done, tokens, targets):
+            if targets.shape != tokens.shape:
+                raise ValueError("not for this objective")
+            return (model(tokens) * targets.sum()).sum()
+
+    step.objective = Objective()
+    return step
+
+
+def test_recording_writes_into_the_arena_after_gradients_were_dropped(host_step):
+    """``zero_grad()`` drops the gradients by default: the recorded backward pass must fill the arena all the same."""
+    step = host_step
+    step.model.zero_grad()
+    step._capture(torch.ones(5, 3), torch.ones(5, 3))
+    assert all(p.grad is view for p, view in zip(step.arena.params, step.arena.views))
+    assert all(bool(view.any()) for view in step.arena.views)
