@@ -604,11 +604,12 @@ class QLoRAStep:
         the recording (the kernels take raw pointers and never allocate or synchronise, so they are capture-safe)."""
         self._hold(*inputs)
         self.arena.rebind()          # stand-ins begin with the gradients that their parameters have
-        self._graph = torch.cuda.CUDAGraph()
+        graph = torch.cuda.CUDAGraph()
         lib = _native.library()
         before = lib.molt_launch_count()
-        with leaves_of_its_own(self.model), torch.cuda.graph(self._graph):
-            self._static_loss = self._forward_backward(*self._static_inputs)
+        with leaves_of_its_own(self.model), torch.cuda.graph(graph):
+            loss = self._forward_backward(*self._static_inputs)
+        self._graph, self._static_loss = graph, loss   # only now: a recording that raises leaves none behind
         self.graph_launches = int(lib.molt_launch_count() - before)   # library kernels recorded; each replay runs them
 
     def _hold(self, *inputs) -> None:

@@ -127,3 +127,13 @@ def test_recording_writes_into_the_arena_after_gradients_were_dropped(host_step)
     step._capture(torch.ones(5, 3), torch.ones(5, 3))
     assert all(p.grad is view for p, view in zip(step.arena.params, step.arena.views))
     assert all(bool(view.any()) for view in step.arena.views)
+
+
+def test_recording_that_failed_leaves_none_behind(host_step):
+    """Inputs that the objective refuses: the next step records anew instead of replaying nothing."""
+    step = host_step
+    with pytest.raises(ValueError, match="not for this objective"):
+        step._capture(torch.ones(5, 3), torch.ones(4, 3))
+    assert step._graph is None and step._static_loss is None
+    step._capture(torch.ones(5, 3), torch.ones(5, 3))
+    assert isinstance(step._graph, _Recording) and step._static_loss is not None

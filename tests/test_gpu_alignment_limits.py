@@ -178,3 +178,25 @@ def test_captured_step_runs_the_hooks_of_its_parameters(native_library):
         assert (step.replayed_launches > 0) == graph
         runs.append(torch.stack(grads))
     assert torch.equal(*runs)
+
+
+def test_step_records_again_after_inputs_that_were_refused(native_library):
+    """The third step, which is the recorded one, is given an odd number of sequences; the fourth is right again."""
+    from molt_b200.qlora_step import DecoderShape, PreferenceObjective, QLoRAStep
+
+    shape = DecoderShape(layers=1, hidden=128, heads=4, kv_heads=2, head_dim=32, intermediate=256, vocab=512, rope_theta=1e4,
+                         rank=8, alpha=16.0, nested_absmax=True, seq_len=32, micro_batch=2)
+    runs = []
+    for graph in (False, True):
+        step = QLoRAStep(shape, torch.device("cuda"), lr=1e-3, objective=PreferenceObjective(), cuda_graph=graph)
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        losses = []
+        for i in range(5):
+            tokens = torch.randint(0, 512, (2, 32), device="cuda", generator=gen)
+            if i == 2:
+                with pytest.raises(ValueError, match="chosen sequences"):
+                    step.run(tokens[:1], tokens[:1])
+            losses.append(step.run(tokens, tokens.roll(-1, 1)).clone())
+        assert (step.replayed_launches > 0) == graph
+        runs.append((torch.stack(losses), step.optimizer.flat.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
