@@ -15,6 +15,7 @@ from pathlib import Path
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from molt_b200.core.errors import CapabilityError
 
@@ -251,6 +252,13 @@ _HERE = nullcontext()
 def on_device(device: torch.device):
     """Context in which ``device`` is the current one; costs next to nothing where it is already."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def refuse_tangents(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raise for dual tensors, as torch does for a custom function without a forward-mode derivative: callers that pass the
+    autograd node by, or take raw pointers, would drop their tangents."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no forward-mode derivative")
 
 
 def ptr(tensor: Optional[torch.Tensor]) -> Optional[int]:

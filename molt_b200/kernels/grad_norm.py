@@ -52,6 +52,7 @@ def _check_device(grads: Tuple[torch.Tensor, ...]) -> None:
 
 def _launch(grads: Tuple[torch.Tensor, ...], outs: Optional[Tuple[torch.Tensor, ...]], kind: int, max_norm: float) -> torch.Tensor:
     _check_device(grads)
+    _native.refuse_tangents("the gradient norm", *grads)
     items, device, count = _native.grad_items(grads, outs), grads[0].device, len(grads)
     lib = _native.library()
     scratch = _native.workspace(lib.molt_grad_norm_workspace_bytes(count), device)

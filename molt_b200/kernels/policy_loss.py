@@ -136,6 +136,7 @@ def clipped_policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
     _check_mask(mask, logprobs)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    _native.refuse_tangents("clipped_policy_loss", logprobs, old_logprobs, advantages, ref_logprobs)
     call = (old_logprobs, ref_logprobs, advantages, mask, float(clip_low), float(clip_high), float(kl_coef),
             _REDUCTIONS[reduction])
     if logprobs.requires_grad and torch.is_grad_enabled():
@@ -213,6 +214,7 @@ def preference_loss(logprobs: torch.Tensor, ref_logprobs: Optional[torch.Tensor]
     _check_mask(mask, logprobs)
     if kind not in _KINDS:
         raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+    _native.refuse_tangents("preference_loss", logprobs, ref_logprobs)
     call = (ref_logprobs, mask, float(beta), float(label_smoothing), _KINDS[kind], int(bool(average)))
     if logprobs.requires_grad and torch.is_grad_enabled():
         told: list = []

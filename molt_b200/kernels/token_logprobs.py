@@ -93,6 +93,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, temperature: f
     outside ``[0, vocab)`` (an ignore index such as -100) gives 0 and no gradient, whatever its row holds.  Logits of -inf
     have probability zero; a row without a finite logit, or with a NaN or +inf, gives NaN."""
     _check(logits, token_ids)
+    _native.refuse_tangents("token_logprobs", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogprobs.apply(logits, token_ids, float(temperature))
     return _forward(*_read_where_it_is(logits), token_ids.contiguous(), float(temperature), None)
@@ -108,6 +109,7 @@ def token_logprobs_with_grad(logits: torch.Tensor, token_ids: torch.Tensor, weig
     be ``logits`` itself, which it then overwrites (it must not overlap them in any other way).  Nothing is recorded for
     autograd."""
     dtype = _check(logits, token_ids)
+    _native.refuse_tangents("token_logprobs_with_grad", logits, weight, out)
     (rows, layout), ids = _read_where_it_is(logits.detach()), token_ids.contiguous()
     if weight is not None:
         if weight.shape != token_ids.shape or weight.dtype != torch.float32 or weight.device != logits.device:

@@ -385,6 +385,7 @@ def frozen_head_logprobs(hidden: torch.Tensor, head: torch.Tensor, token_ids: to
         raise CapabilityError("frozen_head_logprobs requires CUDA tensors")
     if chunk < 1:
         raise ValueError("chunk must be positive")
+    _native.refuse_tangents("frozen_head_logprobs", hidden, head)
     trained = hidden.requires_grad and torch.is_grad_enabled()
     return _FrozenHeadLogprobs.apply(hidden, head, token_ids, int(chunk), float(temperature), trained)
 

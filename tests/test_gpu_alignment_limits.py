@@ -28,11 +28,11 @@ def test_policy_loss_keeps_a_nan_beside_an_advantage_of_zero(native_library, bat
     for reduction in ("token", "sequence"):
         got = clipped_policy_loss(leaf, given["old_logprobs"], torch.zeros(batch, device="cuda"), mask, reduction=reduction)
         (grad,) = torch.autograd.grad(got.loss, leaf)
-        assert math.isnan(float(got.loss)) != masked and math.isnan(float(grad[0, 0])) != masked
+        assert math.isnan(float(got.loss.detach())) != masked and math.isnan(float(grad[0, 0])) != masked
         grad[0, 0] = 0.0
         assert not bool(grad.any())
         if masked:
-            assert float(got.loss) == 0.0
+            assert float(got.loss.detach()) == 0.0
         assert float(got.clip_fraction) == 0.0
 
 
@@ -54,7 +54,7 @@ def test_preference_loss_of_sequences_without_probability(native_library, pairs,
         against = smoothing if side == "rejected" else 1.0 - smoothing          # the factor of the infinite term
         want = math.inf if against else one * (pairs - 1) / pairs
         # the loss is summed in 64 bits and rounded once, the logarithm above is off by 2^-53
-        assert float(got.loss) == pytest.approx(want, rel=2.0 ** -23, abs=0.0)
+        assert float(got.loss.detach()) == pytest.approx(want, rel=2.0 ** -23, abs=0.0)
         slope = (beta * smoothing if side == "rejected" else -beta * (1.0 - smoothing)) / pairs
         for row, sign in ((0, 1.0), (pairs, -1.0)):
             assert torch.equal(grad[row], grad[row, :1].expand(seq))
@@ -200,3 +200,32 @@ def test_step_records_again_after_inputs_that_were_refused(native_library):
         assert (step.replayed_launches > 0) == graph
         runs.append((torch.stack(losses), step.optimizer.flat.clone()))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_dual_tensors_are_refused(native_library):
+    """Nothing here has a forward-mode derivative: a tangent must not be dropped without a word, with or without grad mode,
+    and for the losses' other arguments neither."""
+    import torch.autograd.forward_ad as fwd
+
+    from molt_b200 import kernels
+    from molt_b200.qlora_step import frozen_head_logprobs
+
+    logits, ids = torch.randn(4, 64, device="cuda"), torch.randint(0, 64, (4,), device="cuda")
+    lp, adv = torch.randn(4, 6, device="cuda"), torch.randn(4, device="cuda")
+    hidden, head = torch.randn(4, 64, device="cuda").bfloat16(), torch.randn(64, 64, device="cuda").bfloat16()
+    calls = [(logits, lambda d: kernels.token_logprobs(d, ids)), (logits, lambda d: kernels.token_logprobs_with_grad(d, ids)),
+             (adv, lambda d: kernels.token_logprobs_with_grad(logits, ids, d)),
+             (lp, lambda d: kernels.clipped_policy_loss(d, lp, adv)), (lp, lambda d: kernels.clipped_policy_loss(lp, d, adv)),
+             (adv, lambda d: kernels.clipped_policy_loss(lp, lp, d)),
+             (lp, lambda d: kernels.clipped_policy_loss(lp, lp, adv, ref_logprobs=d)),
+             (lp, lambda d: kernels.preference_loss(d)), (lp, lambda d: kernels.preference_loss(lp, d)),
+             (lp, lambda d: kernels.global_grad_norm([adv, d])), (lp, lambda d: kernels.clip_grad_norm([d, adv], 1.0)),
+             (hidden, lambda d: frozen_head_logprobs(d, head, ids)), (head, lambda d: frozen_head_logprobs(hidden, d, ids))]
+    for primal, call in calls:
+        for tracked in (False, True):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with fwd.dual_level(), mode():
+                    dual = fwd.make_dual(primal.clone().requires_grad_(tracked and primal is not head), torch.ones_like(primal))
+                    with pytest.raises(NotImplementedError):
+                        call(dual)
+                    call(primal.clone())                  # a tensor without a tangent is welcome inside the level
