@@ -242,6 +242,8 @@ def check(code: int) -> None:
 def stream_handle(device: Optional[torch.device] = None) -> int:
     if device is not None and not isinstance(device, torch.device):
         device = torch.device(device)
+    if device is not None and device.type != "cuda":
+        raise ValueError(f"expected a cuda device, not {device}")
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)   # no Stream object: this stands in front of every call
 

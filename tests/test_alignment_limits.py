@@ -137,3 +137,13 @@ def test_recording_that_failed_leaves_none_behind(host_step):
     assert step._graph is None and step._static_loss is None
     step._capture(torch.ones(5, 3), torch.ones(5, 3))
     assert isinstance(step._graph, _Recording) and step._static_loss is not None
+
+
+def test_no_stream_is_named_for_a_device_that_is_not_cuda(monkeypatch):
+    """A host tensor must not reach a kernel by way of the current device's stream."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 40 + index, raising=False)
+    for device in (torch.device("cpu"), "cpu", torch.device("meta")):
+        with pytest.raises(ValueError, match="cuda"):
+            _native.stream_handle(device)
+    assert [_native.stream_handle(d) for d in (None, "cuda", torch.device("cuda:1"), "cuda:2")] == [40, 40, 41, 42]
