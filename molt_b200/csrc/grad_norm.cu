@@ -166,7 +166,7 @@ __device__ __forceinline__ double chunk_total(const T* g, int n, double acc) {
   return acc;
 }
 
-// HBM-bound: 742 MB in 84 tensors take 112 us (6.6 TB/s), a 74 MB arena 14.7 us.  8 loads in flight per thread, 4096 or 16384
+// HBM-bound: 742 MB in 84 tensors take 112 us (6.6 TB/s), a 74 MB arena 14.7 us (8.5 where the L2 holds it already).  8 loads in flight per thread, 4096 or 16384
 // elements per chunk and more blocks were each within 5 %, or slower.
 template <bool MAX, int CAPACITY>
 __global__ void __launch_bounds__(kThreads, 5) norm_kernel(const __grid_constant__ Table<CAPACITY> table,

@@ -2,10 +2,11 @@
 // One pass over a few fp32 arrays of [batch, seq].  The weights of the mean are only known once all masks have been counted,
 // and the scale of the gradient arrives with the backward pass, so the forward writes the gradient without either and the
 // backward multiplies both in (29 bytes per token in all with a reference; recomputing in the backward would move 38).
-// What bounds them: small batches the launches (one for a forward of at most 8192 tokens, 6.5 us; 3 us for a backward);
-// 512 x 4096 tokens the arithmetic of about 125 instructions per token and the latency of one wave of blocks (policy forward
-// 15 us where the bytes would take 5, preference forward 11 us for twice the tokens); 2048 x 4096 tokens HBM to about a half
-// (46 us policy, 17 us preference, 9-11 us backward).
+// What bounds them (device time a call, forward alone, calls replayed one behind the other): small batches the launches (one for
+// a forward of at most 8192 tokens, policy 5.6 us and preference 4; 3 us for a backward); 512 x 4096 tokens the arithmetic of
+// about 125 instructions per token and the latency of one wave of blocks (policy 17 us where the bytes would take 5, preference
+// 10 us for twice the tokens); 2048 x 4096 tokens HBM to about a half (policy 40 us, preference 14, backward 9-11); tens of
+// thousands of pairs their one finishing block (32768 pairs: 112 us).
 #include <math.h>
 
 #include <type_traits>

@@ -337,7 +337,7 @@ __device__ __forceinline__ void copy_wait() {
 // it still holds.  The ring is unrolled and the cluster's size a constant, so that a batch of 16 elements costs few
 // instructions beside its arithmetic (27 per pair of elements in all; 38 with computed slots and addresses, which took
 // 225 us and drew more power).  2048 rows of 151936 bf16: 212 us, 205 in place, where a copy of the same bytes takes 195;
-// 8192 rows 0.81 ms, and 0.88-0.91 in a long loop, when the power cap lowers the clock.  Other forms, same 2048 rows: loads
+// 8192 rows 0.81 ms in a short run of calls, 0.84-0.95 in long ones, by how far the power cap lowers the clock.  Other forms, same 2048 rows: loads
 // through registers 232 us, rows held in the registers of a cluster 291-388, in its shared memory 253-390 (the join of the
 // row then leaves the memory idle), persistent blocks that fetch their next row early 231-296, two kernels (forward, then
 // backward_kernel) 280.
